@@ -26,6 +26,13 @@ __all__ = [
     "attention_decode_fp8",
     "attention_decode_paged",
     "attention_decode_partial",
+    "attention_prefill",
+    "attention_prefill_paged",
+    "cache_compact",
+    "cache_copy_pages",
+    "cache_fork",
+    "cache_resize",
+    "cache_write",
     "combine_partials",
     "workspace_bytes",
     "read_error_flag",
@@ -460,8 +467,132 @@ def combine_partials(acc, ml, out=None):
     return out
 
 
+def _tensors(**named):
+    Tensor = _torch().Tensor
+    for name, t in named.items():
+        if not isinstance(t, Tensor):
+            raise TypeError(f"{name} must be a tensor")
+
+
+def _nhd(layout) -> bool:
+    if layout not in _PAGED_LAYOUTS:
+        raise ValueError(f"layout must be 'HND' or 'NHD' (got {layout!r})")
+    return layout == "NHD"
+
+
+def attention_prefill(q, k, v, cu_seqlens):
+    """Causal attention of whole prompts, packed one behind another.
+
+    Q: [T,Hq,D], K/V: [T,Hkv,D], BF16; D is 64 or 128 and Hq/Hkv 1 to 64.
+    ``cu_seqlens``: int32 [B+1] on the device, ascending from 0: sequence b has
+    rows ``cu_seqlens[b]`` to ``cu_seqlens[b+1] - 1`` (empty ones are allowed)
+    and its token i attends to its tokens 0 to i.  Rows behind the last
+    sequence are padding and come back as zeros.  The tensors may be views
+    (of a fused projection, say) whose token and head strides and offset are
+    multiples of 8 elements.  Returns a new contiguous [T,Hq,D] BF16 tensor.
+    Uses the current CUDA stream.
+    """
+    _tensors(Q=q, K=k, V=v, cu_seqlens=cu_seqlens)
+    return _get_extension().prefill(q, k, v, cu_seqlens)
+
+
+def attention_prefill_paged(q, k_cache, v_cache, block_table, cu_seqlens, seqlens, *, layout="HND"):
+    """Causal attention of new tokens over a paged cache that already holds
+    them (:func:`cache_write`): chunks of a long prompt, prompts behind a
+    shared prefix, drafted tokens, single tokens, or all of them in one batch.
+
+    Q: [T,Hq,D] BF16, the new tokens of the B rows of ``block_table`` packed as
+    ``cu_seqlens`` (int32 [B+1]) says.  ``seqlens`` (int32 [B]) counts a row's
+    cached tokens, the new ones included: with n new tokens, token i attends
+    to the row's tokens 0 to ``seqlens[b] - n + i``; one that sees no token
+    gives zeros, and so does padding behind the last row.  Caches,
+    ``block_table`` and ``layout`` as for :func:`attention_decode_paged`, with
+    Hq/Hkv from 1 to 64.  Returns a new contiguous [T,Hq,D] BF16 tensor.
+    """
+    _tensors(Q=q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, cu_seqlens=cu_seqlens, seqlens=seqlens)
+    return _get_extension().prefill_paged(q, k_cache, v_cache, block_table, cu_seqlens, seqlens, _nhd(layout))
+
+
+def cache_write(k, v, k_cache, v_cache, block_table, cu_seqlens, starts, *, layout="HND"):
+    """Writes new tokens' K and V ([T,Hkv,D] BF16, packed as ``cu_seqlens``
+    says) into the pages of their rows: token i of row b goes to position
+    ``starts[b] + i`` (int32 [B]: the tokens that the row held before).
+
+    A token whose position has no page is left out and sets bit 16 of
+    :func:`read_error_flag`.  Other slots, and so pages that rows share in
+    full, are not touched.
+    """
+    _tensors(K=k, V=v, k_cache=k_cache, v_cache=v_cache, block_table=block_table, cu_seqlens=cu_seqlens, starts=starts)
+    _get_extension().cache_write(k, v, k_cache, v_cache, block_table, cu_seqlens, starts, _nhd(layout))
+
+
+def cache_copy_pages(k_cache, v_cache, src, dst):
+    """Copies page ``src[i]`` of both pools over page ``dst[i]`` (int32 [n] on
+    the device, either layout): the copies that :func:`cache_fork` and
+    :func:`cache_compact` ask for, once per layer.
+
+    An entry of -1 means no copy; other entries outside the pool are left out
+    and set bit 16 of :func:`read_error_flag`.  The copies run side by side,
+    so a page may be the source of several, but the destination of one only,
+    and no destination may be a source.
+    """
+    _tensors(k_cache=k_cache, v_cache=v_cache, src=src, dst=dst)
+    _get_extension().cache_copy_pages(k_cache, v_cache, src, dst)
+
+
+def cache_resize(block_table, seqlens, new_lens, page_refs, *, page_size):
+    """Gives each row of ``block_table`` the pages for ``new_lens[b]`` tokens,
+    in place; ``seqlens`` are the lengths before.  Returns the lengths after
+    (int32 [B]); nothing waits for the device.
+
+    ``page_refs`` (int32 [num_blocks]) counts the rows that hold a page; a
+    free page has 0.  Entries behind a row's pages are -1.  Rows with a new
+    length of 0 let their pages go first, then rows that get shorter; then the
+    growing rows, in row order, take the lowest free pages.  A row that no
+    longer fits, and every later one that needs a page, keeps its length (bit
+    32 of :func:`read_error_flag`).  A length that is negative or larger than
+    the row has entries for is refused, and so is a cut that leaves a partly
+    used page which another row holds, since its next token would overwrite
+    the other's (bit 64).  At most 16384 rows.
+    """
+    _tensors(block_table=block_table, seqlens=seqlens, new_lens=new_lens, page_refs=page_refs)
+    return _get_extension().cache_resize(block_table, seqlens, new_lens, page_refs, page_size)
+
+
+def cache_fork(block_table, seqlens, page_refs, parents, children, *, page_size):
+    """Makes row ``children[i]``, which has to be empty, a copy of row
+    ``parents[i]`` (int32 [n]) in ``block_table`` and ``page_refs``, in place.
+
+    A child shares its parent's full pages; for a partly filled last page it
+    takes the lowest free one, into which the caller copies the parent's:
+    ``lens, src, dst = cache_fork(...)``, then :func:`cache_copy_pages` with
+    ``src, dst`` (int32 [n], -1 where there is nothing to copy) for each
+    layer.  ``lens`` are the lengths after.  Parents' lengths are those before
+    the call.  A row index outside the table, a child that is not empty or
+    was named before is refused (bit 64 of :func:`read_error_flag`); where no
+    free page is left the child stays empty (bit 32).
+    """
+    _tensors(block_table=block_table, seqlens=seqlens, page_refs=page_refs, parents=parents, children=children)
+    return _get_extension().cache_fork(block_table, seqlens, page_refs, parents, children, page_size)
+
+
+def cache_compact(block_table, seqlens, page_refs, *, page_size):
+    """Brings the live pages to the front of the pool with the fewest copies:
+    of n live pages, those at or above n go, in order, to the free ones below.
+
+    ``block_table`` and ``page_refs`` name the new places when the call is
+    done; ``src, dst = cache_compact(...)`` (int32 [num_blocks // 2], -1
+    behind the last) are the copies that the caller makes for each layer
+    (:func:`cache_copy_pages`) before it reads or writes the caches again.
+    """
+    _tensors(block_table=block_table, seqlens=seqlens, page_refs=page_refs)
+    return _get_extension().cache_compact(block_table, seqlens, page_refs, page_size)
+
+
 def read_error_flag(device=0, reset=True) -> int:
-    """Sticky device error word (non-zero if a kernel's bounded wait expired)."""
+    """Sticky device error word: non-zero if a kernel's bounded wait expired
+    (1, 4), a cache had no room (8, 32) or a cache call's device data could not
+    be followed (16, 64)."""
     lib = _lib.load_library()
     flag = ctypes.c_int(0)
     _lib.check(lib, lib.adb_read_error_flag(device, ctypes.byref(flag), int(bool(reset))))

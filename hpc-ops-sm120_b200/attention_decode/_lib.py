@@ -30,6 +30,9 @@ ADB_PAGED_HND = 0
 ADB_PAGED_NHD = 1
 ADB_ERROR_FLAG_PEER_TIMEOUT = 4
 ADB_ERROR_FLAG_APPEND_FULL = 8
+ADB_ERROR_FLAG_CACHE_PAGE = 16
+ADB_ERROR_FLAG_CACHE_FULL = 32
+ADB_ERROR_FLAG_CACHE_REFUSED = 64
 
 STATUS_NAMES = {
     ADB_OK: "ok",
@@ -98,6 +101,30 @@ PROTOTYPES = {
         [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_vp), _int, _int,
          _vp, _i64, _vp, ctypes.c_size_t, ctypes.c_uint, _int, _vp],
     ),
+    "adb_prefill_workspace_size": (
+        _int, [_i64, _i64, _i64, _i64, _i64, _int, ctypes.POINTER(_size), ctypes.POINTER(_size)],
+    ),
+    "adb_prefill": (
+        _int,
+        [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
+         _vp, _size, _uint, _int, _vp],
+    ),
+    "adb_prefill_paged": (
+        _int,
+        [_vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+         _int, _vp, _size, _uint, _int, _vp],
+    ),
+    "adb_cache_write": (
+        _int,
+        [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64,
+         _i64, _int, _int, _vp],
+    ),
+    "adb_cache_copy_pages": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp]),
+    "adb_cache_resize": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _vp]),
+    "adb_cache_fork": (
+        _int, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _vp],
+    ),
+    "adb_cache_compact": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _vp]),
     "adb_read_error_flag": (_int, [_int, ctypes.POINTER(_int), _int]),
     "adb_launch_count": (_int, [ctypes.POINTER(_i64)]),
     "adb_timing_enable": (_int, [_int]),

@@ -3,7 +3,8 @@ PyTorch C++ extension adb_torch_ext.so over it.
 
     python hpc-ops-sm120_b200/build_lib.py [--force] [--verbose]
 
-The library is one translation unit (csrc/decode_capi.cu) with the CUDA
+The library is three translation units (csrc/decode_capi.cu, cache_capi.cu
+and prefill_capi.cu, compiled side by side) with the CUDA
 runtime linked statically and the driver's tensor-map encoder fetched at run
 time, so it depends on nothing but libc/libstdc++ and loads on machines
 without a GPU.  The extension (csrc/torch_binding.cpp) holds no kernels: it
@@ -26,8 +27,15 @@ ROOT = PACKAGE_DIR.parent
 CSRC = PACKAGE_DIR / "csrc"
 INCLUDE = ROOT / "include"
 OUTPUT = PACKAGE_DIR / "attention_decode" / "libattention_decode_b200.so"
-SOURCES = [CSRC / "decode_capi.cu"]
-DEPENDENCIES = SOURCES + sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*.h"))
+SHARED = [CSRC / "device_primitives.cuh", CSRC / "host_common.h", *sorted(INCLUDE.glob("*.h"))]
+# each source with the headers of its own
+UNITS = {
+    CSRC / "decode_capi.cu": [CSRC / "decode_kernels.cuh"],
+    CSRC / "cache_capi.cu": [CSRC / "cache_kernels.cuh"],
+    CSRC / "prefill_capi.cu": [CSRC / "prefill_kernels.cuh"],
+}
+SOURCES = list(UNITS)
+DEPENDENCIES = SOURCES + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + sorted(INCLUDE.glob("*.h"))
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -36,8 +44,10 @@ NVCC_FLAGS = [
     "-std=c++17",
     "-Xcompiler", "-fPIC",
     "-Xcompiler", "-fvisibility=hidden",
-    "-shared",
     "-cudart", "static",
+]
+LINK_FLAGS = [
+    "-shared",
     "-Xlinker", "-soname=libattention_decode_b200.so",
 ]
 
@@ -75,14 +85,34 @@ def build(force: bool = False, verbose: bool = False, trace: bool = False) -> Pa
     if not force and up_to_date(output):
         return output
     output.parent.mkdir(parents=True, exist_ok=True)
+    objects = PACKAGE_DIR / "_build" / ("trace_obj" if trace else "obj")
+    objects.mkdir(parents=True, exist_ok=True)
     extra = ["-DADB_TRACE"] if trace else []
-    cmd = [nvcc_path(), *NVCC_FLAGS, *extra, f"-I{INCLUDE}", f"-I{CSRC}", *map(str, SOURCES), "-o", str(output) + ".tmp"]
     if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-        print(" ".join(cmd), flush=True)
-    result = subprocess.run(cmd, capture_output=not verbose, text=True)
+        extra.append("-Xptxas=-v")
+    running = []
+    for source, headers in UNITS.items():
+        obj = objects / f"{source.stem}.o"
+        if force or not up_to_date(obj, [source, *headers, *SHARED]):
+            cmd = [nvcc_path(), *NVCC_FLAGS, *extra, f"-I{INCLUDE}", f"-I{CSRC}", "-c", str(source), "-o", str(obj)]
+            if verbose:
+                print(" ".join(cmd), flush=True)
+            running.append((obj, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    failed = []
+    for obj, process in running:
+        text = process.communicate()[0]
+        if verbose:
+            print(text, flush=True)
+        if process.returncode != 0:
+            obj.unlink(missing_ok=True)
+            failed.append(f"nvcc failed ({process.returncode}):\n{text}")
+    if failed:
+        raise RuntimeError("\n".join(failed))
+    linked = [str(objects / f"{source.stem}.o") for source in UNITS]
+    cmd = [nvcc_path(), *NVCC_FLAGS, *LINK_FLAGS, *linked, "-o", str(output) + ".tmp"]
+    result = subprocess.run(cmd, capture_output=True, text=True)
     if result.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({result.returncode}):\n{result.stdout}\n{result.stderr}")
+        raise RuntimeError(f"link failed ({result.returncode}):\n{result.stdout}\n{result.stderr}")
     os.replace(str(output) + ".tmp", output)
     return output
 

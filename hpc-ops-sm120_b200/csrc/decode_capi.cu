@@ -23,11 +23,18 @@
 
 #include "attention_decode_b200.h"
 #include "decode_kernels.cuh"
+#include "host_common.h"
 
 namespace {
 
 thread_local std::string t_last_error;
 std::atomic<int64_t> g_launches{0};
+
+using adb_host::cuda_fail;
+using adb_host::DeviceGuard;
+using adb_host::fail;
+using adb_host::get_encoder;
+using adb_host::is_aligned;
 
 // Per-thread diagnostic timing of the streaming kernel (adb_timing_*).
 struct Timing {
@@ -35,6 +42,10 @@ struct Timing {
   std::vector<std::pair<cudaEvent_t, cudaEvent_t>> events;
 };
 thread_local Timing t_timing;
+
+}  // namespace
+
+namespace adb_host {
 
 int fail(int code, const char* fmt, ...) {
   char buf[512];
@@ -49,6 +60,10 @@ int fail(int code, const char* fmt, ...) {
 int cuda_fail(cudaError_t e, const char* what) {
   return fail(ADB_ERR_CUDA, "%s: %s (%s)", what, cudaGetErrorString(e), cudaGetErrorName(e));
 }
+
+}  // namespace adb_host
+
+namespace {
 
 // ------------------------------------------------------------ kernel table
 struct Variant {
@@ -198,6 +213,10 @@ PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 std::once_flag g_encode_once;
 cudaError_t g_encode_error = cudaSuccess;
 
+}  // namespace
+
+namespace adb_host {
+
 int get_encoder(PFN_cuTensorMapEncodeTiled_v12000* fn) {
   std::call_once(g_encode_once, [] {
     void* ptr = nullptr;
@@ -214,6 +233,19 @@ int get_encoder(PFN_cuTensorMapEncodeTiled_v12000* fn) {
   *fn = g_encode;
   return ADB_OK;
 }
+
+int sm_count(int device, int* sms) {
+  DeviceState* st = nullptr;
+  const int rc = probe_device(device, &st);
+  if (rc == ADB_OK) *sms = st->sms;
+  return rc;
+}
+
+void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
+
+}  // namespace adb_host
+
+namespace {
 
 // 3-D map over one KV tensor viewed as [pairs][S][D] bf16; a box is
 // 64 columns (128 bytes, swizzled) x tile_tokens rows x 1 pair.  Rows past S
@@ -385,24 +417,6 @@ int make_plan(const Shape& s, bool varlen, bool tma, DeviceState* st, Plan* plan
   plan->bytes = plan->off_ml + align256(slots * s.G * 2 * sizeof(float));
   return ADB_OK;
 }
-
-struct DeviceGuard {
-  int previous = -1;
-  bool switched = false;
-  cudaError_t error = cudaSuccess;
-  explicit DeviceGuard(int device) {
-    error = cudaGetDevice(&previous);
-    if (error == cudaSuccess && previous != device) {
-      error = cudaSetDevice(device);
-      switched = error == cudaSuccess;
-    }
-  }
-  ~DeviceGuard() {
-    if (switched) cudaSetDevice(previous);
-  }
-};
-
-bool is_aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
 // A paged K/V cache (adb_decode_paged): pools of 2^page_shift-token pages.
 struct PagedArgs {
@@ -984,6 +998,13 @@ int adb_read_error_flag(int device, int* flag, int reset) {
     const int zero = 0;
     e = cudaMemcpyToSymbol(adb::g_adb_error_flag, &zero, sizeof(int));
     if (e != cudaSuccess) return cuda_fail(e, "clearing the device error flag");
+  }
+  // Each translation unit with kernels has an error word of its own.
+  for (auto read : {adb_host::cache_error_word, adb_host::prefill_error_word}) {
+    int word = 0;
+    e = read(&word, reset != 0);
+    if (e != cudaSuccess) return cuda_fail(e, "reading the device error flag");
+    *flag |= word;
   }
   return ADB_OK;
 }

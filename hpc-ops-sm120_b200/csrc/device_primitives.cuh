@@ -62,14 +62,18 @@ __device__ __forceinline__ uint64_t global_timer_ns() {
   return t;
 }
 
-// Sticky per-device error word, set when a bounded wait gives up.  Defined
-// here: the library is one translation unit (decode_capi.cu).
-__device__ int g_adb_error_flag = 0;
+// Sticky per-device error word, set when a bounded wait gives up or a call's
+// device data cannot be followed.  One per translation unit;
+// adb_read_error_flag returns their union.
+static __device__ int g_adb_error_flag = 0;
 
 constexpr int kErrWaitTimeout = 1;
 constexpr int kErrWorkspace = 2;  // a scheduler counter left its bounds (dirty header)
 constexpr int kErrPeerTimeout = 4;  // a peer's partial states did not arrive in time
 constexpr int kErrAppendFull = 8;   // append: a sequence's cache had no free position
+constexpr int kErrCachePage = 16;   // a table entry or page index outside the pool
+constexpr int kErrCacheFull = 32;   // resize / fork: no free page left for a row
+constexpr int kErrCacheRefused = 64;  // resize / fork: a row's request was refused
 constexpr uint64_t kWaitLimitNs = 2000000000ull;  // 2 s: far above any legitimate wait
 
 // Waits for the given phase parity of an mbarrier.  The wait is bounded: if

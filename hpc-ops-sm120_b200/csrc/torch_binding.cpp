@@ -11,7 +11,8 @@
 //
 // Additions, all compatible with the 3-argument call: an optional int32
 // `seqlens` [B] on forward, forward_partial (unnormalised (acc, m, l) states
-// for sequence sharding) and combine (merge of R such states).
+// for sequence sharding) and combine (merge of R such states); prompt attention
+// (prefill, prefill_paged) and the upkeep of a paged cache (cache_*).
 #include <torch/extension.h>
 
 #include <ATen/cuda/CUDAContext.h>
@@ -20,6 +21,7 @@
 
 #include <map>
 #include <mutex>
+#include <string>
 #include <utility>
 
 #include "attention_decode_b200.h"
@@ -166,6 +168,235 @@ at::Tensor combine(const at::Tensor& acc, const at::Tensor& ml) {
   return out;
 }
 
+// ---- Prompt attention and paged-cache upkeep.  The checks that need no
+// device come first, that the tensors are on one comes last.
+
+void check_bf16(const at::Tensor& t, const char* name, int64_t rank) {
+  TORCH_CHECK(t.scalar_type() == at::kBFloat16, name, " dtype must be BF16 (bfloat16)");
+  TORCH_CHECK(t.dim() == rank, name, " must have rank ", std::to_string(rank).c_str());
+  TORCH_CHECK(!t.requires_grad(), name, ": forward inference only; no backward/grad support");
+}
+
+void check_int32(const at::Tensor& t, const char* name, int64_t rank) {
+  TORCH_CHECK(t.scalar_type() == at::kInt, name, " dtype must be int32");
+  TORCH_CHECK(t.dim() == rank, name, " must have rank ", std::to_string(rank).c_str());
+  if (rank == 1) {
+    TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+  } else {
+    TORCH_CHECK(t.size(0) > 0 && t.size(1) > 0 && t.stride(1) == 1 && (t.size(0) == 1 || t.stride(0) >= t.size(1)),
+                name, " must have contiguous, distinct rows");
+  }
+}
+
+// A packed [tokens, heads, D] tensor: any token and head stride that keeps
+// 16-byte vectors aligned (views of a fused projection qualify).
+void check_packed(const at::Tensor& t, const char* name) {
+  check_bf16(t, name, 3);
+  TORCH_CHECK(t.size(2) == 64 || t.size(2) == 128, "head dimension must be 64 or 128");
+  TORCH_CHECK(t.size(1) > 0, name, " must have heads");
+  TORCH_CHECK(t.stride(2) == 1, name, " must be contiguous in the head dimension");
+  TORCH_CHECK((t.size(0) <= 1 || t.stride(0) % 8 == 0) && (t.size(1) <= 1 || t.stride(1) % 8 == 0) &&
+                  t.storage_offset() % 8 == 0,
+              name, " must start at, and have token and head strides of, a multiple of 8 elements");
+  TORCH_CHECK((t.size(0) <= 1 || t.stride(0) > 0) && (t.size(1) <= 1 || t.stride(1) > 0), name,
+              " must not be expanded");
+}
+
+// Strides as the C ABI takes them (a stride of a dimension of size 1 may be anything).
+int64_t token_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2); }
+int64_t head_stride(const at::Tensor& t) { return t.size(1) > 1 ? t.stride(1) : t.size(2); }
+
+int64_t row_stride(const at::Tensor& table) { return table.size(0) > 1 ? table.stride(0) : table.size(1); }
+
+struct Pages {
+  int64_t blocks, heads, page, dim;
+  int layout;
+};
+
+Pages check_caches(const at::Tensor& k_cache, const at::Tensor& v_cache, bool nhd) {
+  check_bf16(k_cache, "k_cache", 4);
+  check_bf16(v_cache, "v_cache", 4);
+  TORCH_CHECK(k_cache.sizes() == v_cache.sizes(), "K/V cache shapes must match");
+  TORCH_CHECK(k_cache.is_contiguous() && v_cache.is_contiguous(), "K/V caches must be contiguous");
+  TORCH_CHECK(k_cache.numel() > 0, "empty caches are unsupported");
+  return {k_cache.size(0), k_cache.size(nhd ? 2 : 1), k_cache.size(nhd ? 1 : 2), k_cache.size(3),
+          nhd ? ADB_PAGED_NHD : ADB_PAGED_HND};
+}
+
+void check_batch(const at::Tensor& t, const char* name, int64_t batch) {
+  check_int32(t, name, 1);
+  TORCH_CHECK(t.size(0) == batch, name, " must have ", std::to_string(batch).c_str(), " entries");
+}
+
+// All on the CUDA device of the first (ValueError, as for Q, K and V elsewhere).
+void check_devices(std::initializer_list<std::pair<const char*, const at::Tensor*>> tensors) {
+  const at::Tensor* first = tensors.begin()->second;
+  for (const auto& t : tensors) {
+    TORCH_CHECK_VALUE(t.second->is_cuda(), t.first, " must be a CUDA tensor");
+    TORCH_CHECK(t.second->device() == first->device(), t.first, " must be on the same CUDA device as ",
+                tensors.begin()->first);
+  }
+}
+
+Call prepare_prefill(const at::Tensor& q, int64_t batch, int64_t kv_heads) {
+  const int device = q.get_device();
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream(device).stream();
+  size_t total = 0, header = 0;
+  check_status(adb_prefill_workspace_size(q.size(0), batch, q.size(1), kv_heads, q.size(2), device, &total, &header));
+  return {device, stream, workspace_for(q, device, stream, total, header)};
+}
+
+at::Tensor prefill(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu_seqlens) {
+  check_packed(q, "Q");
+  check_packed(k, "K");
+  check_packed(v, "V");
+  check_int32(cu_seqlens, "cu_seqlens", 1);
+  TORCH_CHECK(cu_seqlens.size(0) >= 1, "cu_seqlens must have batch + 1 entries");
+  TORCH_CHECK(k.sizes() == v.sizes(), "K/V shape must match");
+  TORCH_CHECK(q.size(0) == k.size(0) && q.size(2) == k.size(2), "Q/K/V tokens and head dimension must match");
+  TORCH_CHECK(q.size(1) % k.size(1) == 0, "query heads must be divisible by KV heads");
+  check_devices({{"Q", &q}, {"K", &k}, {"V", &v}, {"cu_seqlens", &cu_seqlens}});
+  const c10::cuda::CUDAGuard guard(q.device());
+  const int64_t batch = cu_seqlens.size(0) - 1;
+  if (q.size(0) == 0 || batch == 0) return at::zeros({q.size(0), q.size(1), q.size(2)}, q.options());
+  at::Tensor out = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
+  Call call = prepare_prefill(q, batch, k.size(1));
+  check_status(adb_prefill(q.data_ptr(), token_stride(q), head_stride(q), k.data_ptr(), token_stride(k),
+                           head_stride(k), v.data_ptr(), token_stride(v), head_stride(v),
+                           cu_seqlens.data_ptr<int32_t>(), out.data_ptr(), q.size(0), batch, q.size(1), k.size(1),
+                           q.size(2), call.ws.buffer.data_ptr(), static_cast<size_t>(call.ws.buffer.numel()),
+                           call.ws.flags, call.device, call.stream));
+  return out;
+}
+
+at::Tensor prefill_paged(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                         const at::Tensor& block_table, const at::Tensor& cu_seqlens, const at::Tensor& seqlens,
+                         bool nhd) {
+  check_packed(q, "Q");
+  const Pages pages = check_caches(k_cache, v_cache, nhd);
+  check_int32(block_table, "block_table", 2);
+  const int64_t batch = block_table.size(0);
+  check_batch(cu_seqlens, "cu_seqlens", batch + 1);
+  check_batch(seqlens, "seqlens", batch);
+  TORCH_CHECK(q.size(2) == pages.dim, "Q and cache head dimension must match");
+  TORCH_CHECK(q.size(1) % pages.heads == 0, "query heads must be divisible by KV heads");
+  check_devices({{"Q", &q}, {"k_cache", &k_cache}, {"v_cache", &v_cache}, {"block_table", &block_table},
+                 {"cu_seqlens", &cu_seqlens}, {"seqlens", &seqlens}});
+  const c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor out = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
+  if (q.size(0) == 0) return out;
+  Call call = prepare_prefill(q, batch, pages.heads);
+  check_status(adb_prefill_paged(
+      q.data_ptr(), token_stride(q), head_stride(q), k_cache.data_ptr(), v_cache.data_ptr(),
+      block_table.data_ptr<int32_t>(), row_stride(block_table),
+      cu_seqlens.data_ptr<int32_t>(), seqlens.data_ptr<int32_t>(), out.data_ptr(), q.size(0), batch, q.size(1),
+      pages.heads, pages.dim, pages.blocks, pages.page, block_table.size(1), pages.layout,
+      call.ws.buffer.data_ptr(), static_cast<size_t>(call.ws.buffer.numel()), call.ws.flags, call.device,
+      call.stream));
+  return out;
+}
+
+void cache_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                 const at::Tensor& block_table, const at::Tensor& cu_seqlens, const at::Tensor& starts, bool nhd) {
+  check_packed(k, "K");
+  check_packed(v, "V");
+  const Pages pages = check_caches(k_cache, v_cache, nhd);
+  TORCH_CHECK(k.sizes() == v.sizes(), "K/V shape must match");
+  TORCH_CHECK(k.size(1) == pages.heads && k.size(2) == pages.dim, "K/V heads and head dimension must match the caches");
+  check_int32(block_table, "block_table", 2);
+  const int64_t batch = block_table.size(0);
+  check_batch(cu_seqlens, "cu_seqlens", batch + 1);
+  check_batch(starts, "starts", batch);
+  check_devices({{"K", &k}, {"V", &v}, {"k_cache", &k_cache}, {"v_cache", &v_cache}, {"block_table", &block_table},
+                 {"cu_seqlens", &cu_seqlens}, {"starts", &starts}});
+  if (k.size(0) == 0) return;
+  const c10::cuda::CUDAGuard guard(k.device());
+  const int device = k.get_device();
+  check_status(adb_cache_write(
+      k.data_ptr(), token_stride(k), head_stride(k), v.data_ptr(), token_stride(v), head_stride(v),
+      k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr<int32_t>(),
+      row_stride(block_table), cu_seqlens.data_ptr<int32_t>(),
+      starts.data_ptr<int32_t>(), k.size(0), batch, pages.heads, pages.dim, pages.blocks, pages.page,
+      block_table.size(1), pages.layout, device, at::cuda::getCurrentCUDAStream(device).stream()));
+}
+
+void cache_copy_pages(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& src,
+                      const at::Tensor& dst) {
+  const Pages pages = check_caches(k_cache, v_cache, false);
+  check_int32(src, "src", 1);
+  check_batch(dst, "dst", src.size(0));
+  check_devices({{"k_cache", &k_cache}, {"v_cache", &v_cache}, {"src", &src}, {"dst", &dst}});
+  if (src.size(0) == 0) return;
+  const c10::cuda::CUDAGuard guard(k_cache.device());
+  const int device = k_cache.get_device();
+  check_status(adb_cache_copy_pages(k_cache.data_ptr(), v_cache.data_ptr(), src.data_ptr<int32_t>(),
+                                    dst.data_ptr<int32_t>(), src.size(0), pages.blocks,
+                                    pages.heads * pages.page * pages.dim * 2, device,
+                                    at::cuda::getCurrentCUDAStream(device).stream()));
+}
+
+void check_book(const at::Tensor& block_table, const at::Tensor& seqlens, const at::Tensor& page_refs) {
+  check_int32(block_table, "block_table", 2);
+  check_batch(seqlens, "seqlens", block_table.size(0));
+  check_int32(page_refs, "page_refs", 1);
+  TORCH_CHECK(page_refs.size(0) > 0, "page_refs must have an entry per page");
+}
+
+at::Tensor cache_resize(const at::Tensor& block_table, const at::Tensor& seqlens, const at::Tensor& new_lens,
+                        const at::Tensor& page_refs, int64_t page_size) {
+  check_book(block_table, seqlens, page_refs);
+  check_batch(new_lens, "new_lens", block_table.size(0));
+  check_devices({{"block_table", &block_table}, {"seqlens", &seqlens}, {"new_lens", &new_lens},
+                 {"page_refs", &page_refs}});
+  const c10::cuda::CUDAGuard guard(block_table.device());
+  const int device = block_table.get_device();
+  at::Tensor lens = at::empty_like(seqlens);
+  check_status(adb_cache_resize(block_table.data_ptr<int32_t>(), row_stride(block_table), seqlens.data_ptr<int32_t>(),
+                                new_lens.data_ptr<int32_t>(), page_refs.data_ptr<int32_t>(), lens.data_ptr<int32_t>(),
+                                block_table.size(0), page_refs.size(0), page_size, block_table.size(1), device,
+                                at::cuda::getCurrentCUDAStream(device).stream()));
+  return lens;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> cache_fork(const at::Tensor& block_table, const at::Tensor& seqlens,
+                                                          const at::Tensor& page_refs, const at::Tensor& parents,
+                                                          const at::Tensor& children, int64_t page_size) {
+  check_book(block_table, seqlens, page_refs);
+  check_int32(parents, "parents", 1);
+  check_batch(children, "children", parents.size(0));
+  check_devices({{"block_table", &block_table}, {"seqlens", &seqlens}, {"page_refs", &page_refs},
+                 {"parents", &parents}, {"children", &children}});
+  const c10::cuda::CUDAGuard guard(block_table.device());
+  const int device = block_table.get_device();
+  at::Tensor src = at::empty_like(parents), dst = at::empty_like(parents);
+  if (parents.size(0) == 0) return {seqlens.clone(), src, dst};
+  at::Tensor lens = at::empty_like(seqlens);
+  check_status(adb_cache_fork(block_table.data_ptr<int32_t>(), row_stride(block_table), seqlens.data_ptr<int32_t>(),
+                              page_refs.data_ptr<int32_t>(), parents.data_ptr<int32_t>(),
+                              children.data_ptr<int32_t>(), parents.size(0), lens.data_ptr<int32_t>(),
+                              src.data_ptr<int32_t>(), dst.data_ptr<int32_t>(), block_table.size(0),
+                              page_refs.size(0), page_size, block_table.size(1), device,
+                              at::cuda::getCurrentCUDAStream(device).stream()));
+  return {lens, src, dst};
+}
+
+std::tuple<at::Tensor, at::Tensor> cache_compact(const at::Tensor& block_table, const at::Tensor& seqlens,
+                                                 const at::Tensor& page_refs, int64_t page_size) {
+  check_book(block_table, seqlens, page_refs);
+  check_devices({{"block_table", &block_table}, {"seqlens", &seqlens}, {"page_refs", &page_refs}});
+  const c10::cuda::CUDAGuard guard(block_table.device());
+  const int device = block_table.get_device();
+  const int64_t blocks = page_refs.size(0);
+  at::Tensor src = at::empty({blocks / 2}, page_refs.options()), dst = at::empty({blocks / 2}, page_refs.options());
+  at::Tensor remap = at::empty({blocks}, page_refs.options());
+  check_status(adb_cache_compact(block_table.data_ptr<int32_t>(), row_stride(block_table),
+                                 seqlens.data_ptr<int32_t>(), page_refs.data_ptr<int32_t>(),
+                                 src.data_ptr<int32_t>(), dst.data_ptr<int32_t>(), remap.data_ptr<int32_t>(),
+                                 block_table.size(0), blocks, page_size, block_table.size(1), device,
+                                 at::cuda::getCurrentCUDAStream(device).stream()));
+  return {src, dst};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -176,4 +407,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         pybind11::arg("q"), pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("seqlens") = pybind11::none());
   m.def("combine", &combine, "merge R partial states into the BF16 output", pybind11::arg("acc"),
         pybind11::arg("ml"));
+  m.def("prefill", &prefill, "causal attention of packed prompts");
+  m.def("prefill_paged", &prefill_paged, "causal attention of new tokens over a paged cache");
+  m.def("cache_write", &cache_write, "new tokens' K and V into their pages");
+  m.def("cache_copy_pages", &cache_copy_pages, "copies of pages inside both pools");
+  m.def("cache_resize", &cache_resize, "pages for new lengths");
+  m.def("cache_fork", &cache_fork, "rows that share their parents' pages");
+  m.def("cache_compact", &cache_compact, "live pages to the front of the pool");
 }

@@ -293,6 +293,118 @@ ADB_API int adb_decode_exchange_merged(const void* q, const void* k, const void*
                                        int64_t timeout_us, void* workspace, size_t workspace_bytes,
                                        unsigned flags, int device, void* stream);
 
+/* ---- Prompt attention and the upkeep of a paged cache (no reference
+ * counterpart: the reference decodes a cache that somebody else filled).
+ *
+ * Packed sequences: the `total` rows of a tensor hold the tokens of `batch`
+ * sequences one behind another; sequence b has rows cu_seqlens[b] to
+ * cu_seqlens[b + 1] - 1 (int32 [batch + 1] on the device, ascending from 0;
+ * empty sequences are allowed).  Rows behind the last sequence are padding.
+ * Token and head strides are in elements and multiples of 8, pointers 16-byte
+ * aligned, the head dimension contiguous. */
+
+#define ADB_ERROR_FLAG_CACHE_PAGE 16    /* a table entry or list entry outside the pool */
+#define ADB_ERROR_FLAG_CACHE_FULL 32    /* no free page left for a row */
+#define ADB_ERROR_FLAG_CACHE_REFUSED 64 /* a row's request was refused */
+
+/* Workspace of adb_prefill and adb_prefill_paged for `total` rows (see
+ * "Workspace" above). */
+ADB_API int adb_prefill_workspace_size(int64_t total, int64_t batch, int64_t q_heads,
+                                       int64_t kv_heads, int64_t head_dim, int device,
+                                       size_t* bytes, size_t* header_bytes);
+
+/* Causal attention of whole prompts.  q [total, q_heads, head_dim], k and v
+ * [total, kv_heads, head_dim], out [total, q_heads, head_dim] contiguous, all
+ * bf16: token i of a sequence attends to the sequence's tokens 0..i.  GQA
+ * groups 1 to 64, head_dim 64 or 128.  Padding rows of out become zero. */
+ADB_API int adb_prefill(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                        int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                        int64_t v_token_stride, int64_t v_head_stride, const int32_t* cu_seqlens,
+                        void* out, int64_t total, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                        int64_t head_dim, void* workspace, size_t workspace_bytes, unsigned flags,
+                        int device, void* stream);
+
+/* Causal attention of new tokens over a paged cache that already holds them
+ * (adb_cache_write): sequence b has seqlens[b] tokens in its pages, the last
+ * n_b = cu_seqlens[b + 1] - cu_seqlens[b] of which are the rows of q, so row i
+ * attends to tokens 0 .. seqlens[b] - n_b + i.  A row before the first token
+ * (seqlens[b] < n_b) becomes zero.  Cache arguments as adb_decode_paged;
+ * tokens whose page is outside the pool count as zeros and set
+ * ADB_ERROR_FLAG_CACHE_PAGE. */
+ADB_API int adb_prefill_paged(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                              const void* k_cache, const void* v_cache, const int32_t* block_table,
+                              int64_t block_table_stride, const int32_t* cu_seqlens,
+                              const int32_t* seqlens, void* out, int64_t total, int64_t batch,
+                              int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                              int64_t num_blocks, int64_t page_size, int64_t max_blocks_per_seq,
+                              int layout, void* workspace, size_t workspace_bytes, unsigned flags,
+                              int device, void* stream);
+
+/* Writes new tokens' K and V into their pages: token i of row b goes to
+ * position starts[b] + i.  A token whose position has no page of the pool is
+ * not written and sets ADB_ERROR_FLAG_CACHE_PAGE.  The slots written must be
+ * distinct (no two rows hold the same page at a position that is written). */
+ADB_API int adb_cache_write(const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                            const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                            void* k_cache, void* v_cache, const int32_t* block_table,
+                            int64_t block_table_stride, const int32_t* cu_seqlens,
+                            const int32_t* starts, int64_t total, int64_t batch, int64_t kv_heads,
+                            int64_t head_dim, int64_t num_blocks, int64_t page_size,
+                            int64_t max_blocks_per_seq, int layout, int device, void* stream);
+
+/* Copies pages inside both pools: page dst[i] gets page src[i]'s bytes.
+ * Entries with a -1 are skipped; other entries outside the pool are skipped
+ * and set ADB_ERROR_FLAG_CACHE_PAGE.  The copies run side by side: a page may
+ * be the source of several, but a destination only once and then no source
+ * (what adb_cache_fork and adb_cache_compact give). */
+ADB_API int adb_cache_copy_pages(void* k_cache, void* v_cache, const int32_t* src,
+                                 const int32_t* dst, int64_t count, int64_t num_blocks,
+                                 int64_t page_bytes, int device, void* stream);
+
+/* The bookkeeping of pages, in device memory: block_table int32 [batch,
+ * max_blocks_per_seq] (rows block_table_stride apart) names the pages that
+ * hold a row's seqlens[b] tokens, -1 behind them; page_refs int32
+ * [num_blocks] counts the rows that hold a page (0: free).  Both are changed
+ * in place; seqlens is not, the lengths after the call go to lens_out.  At
+ * most 16384 rows.  Page sizes as adb_decode_paged.
+ *
+ * adb_cache_resize gives each row the pages for new_lens[b] tokens.  First
+ * the rows with new length 0 let their pages go, then rows that get shorter;
+ * then growing rows, in row order, take the lowest free pages.  A row that no
+ * longer fits, and every later one that needs pages, keeps its length
+ * (ADB_ERROR_FLAG_CACHE_FULL).  A length outside [0, max_blocks_per_seq *
+ * page_size], or a cut that leaves a partly used page which another row
+ * holds, is refused (ADB_ERROR_FLAG_CACHE_REFUSED). */
+ADB_API int adb_cache_resize(int32_t* block_table, int64_t block_table_stride,
+                             const int32_t* seqlens, const int32_t* new_lens, int32_t* page_refs,
+                             int32_t* lens_out, int64_t batch, int64_t num_blocks,
+                             int64_t page_size, int64_t max_blocks_per_seq, int device,
+                             void* stream);
+
+/* adb_cache_fork makes row children[i] a copy of row parents[i] (int32
+ * [forks], at most 16384): it shares the parent's full pages, and for a partly
+ * filled last page takes the lowest free one, whose content the caller copies:
+ * src[i] -> dst[i] (adb_cache_copy_pages, once per layer; -1, -1 where there
+ * is nothing to copy).  Lengths are those before the call.  Refused: a row
+ * index outside the table, a child that is not empty, a child named before.
+ * Forks that find no free page, in order, leave their child empty. */
+ADB_API int adb_cache_fork(int32_t* block_table, int64_t block_table_stride, const int32_t* seqlens,
+                           int32_t* page_refs, const int32_t* parents, const int32_t* children,
+                           int64_t forks, int32_t* lens_out, int32_t* src, int32_t* dst,
+                           int64_t batch, int64_t num_blocks, int64_t page_size,
+                           int64_t max_blocks_per_seq, int device, void* stream);
+
+/* adb_cache_compact brings the n live pages to the front of the pool with the
+ * fewest copies: the i-th live page at or above n goes to the i-th free page
+ * below n.  src and dst (int32 [num_blocks / 2]) list the copies that the
+ * caller makes, then -1; tables and counts already name the new places.
+ * remap: scratch of num_blocks ints. */
+ADB_API int adb_cache_compact(int32_t* block_table, int64_t block_table_stride,
+                              const int32_t* seqlens, int32_t* page_refs, int32_t* src,
+                              int32_t* dst, int32_t* remap, int64_t batch, int64_t num_blocks,
+                              int64_t page_size, int64_t max_blocks_per_seq, int device,
+                              void* stream);
+
 /* Reads (and optionally clears) the sticky device error word that kernels
  * set when a bounded wait gives up; 0 means no kernel has reported an
  * error on `device`.  Synchronous (a device-to-host copy); for diagnostics. */
