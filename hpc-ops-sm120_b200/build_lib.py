@@ -32,7 +32,7 @@ SHARED = [CSRC / "device_primitives.cuh", CSRC / "host_common.h", *sorted(INCLUD
 UNITS = {
     CSRC / "decode_capi.cu": [CSRC / "decode_kernels.cuh"],
     CSRC / "cache_capi.cu": [CSRC / "cache_kernels.cuh"],
-    CSRC / "prefill_capi.cu": [CSRC / "prefill_kernels.cuh"],
+    CSRC / "prefill_capi.cu": [CSRC / "prefill_kernels.cuh", CSRC / "tcgen05_primitives.cuh"],
 }
 SOURCES = list(UNITS)
 DEPENDENCIES = SOURCES + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + sorted(INCLUDE.glob("*.h"))

@@ -2,6 +2,8 @@
 // launches of the kernels in prefill_kernels.cuh.
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "attention_decode_b200.h"
@@ -43,24 +45,100 @@ int check_heads(int64_t total, int64_t batch, int64_t q_heads, int64_t kv_heads,
   return ADB_OK;
 }
 
-int launch(adb::PrefillParams& p, int64_t head_dim, int device, void* stream) {
+// Tensor map over bf16 with a 128-byte swizzle; dims and strides (elements)
+// innermost first, the innermost box always 64 columns.
+int encode(CUtensorMap* map, const void* base, int rank, const int64_t* dims, const int64_t* strides, const int* box) {
+  PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  const int rc = adb_host::get_encoder(&fn);
+  if (rc != ADB_OK) return rc;
+  cuuint64_t d[4], s[3];
+  cuuint32_t b[4], one[4] = {1u, 1u, 1u, 1u};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = static_cast<cuuint64_t>(dims[i]);
+    b[i] = static_cast<cuuint32_t>(box[i]);
+    if (i > 0) s[i - 1] = static_cast<cuuint64_t>(strides[i] * 2);
+  }
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), d, s, b, one,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(ADB_ERR_CUDA, "cuTensorMapEncodeTiled failed (CUresult %d)", int(r));
+  return ADB_OK;
+}
+
+// [tokens][heads][D] with a box of `rows` tokens x `heads_box` heads.
+int encode_packed(CUtensorMap* map, const void* base, int64_t tokens, int64_t heads, int64_t dim, int64_t token_stride,
+                  int64_t head_stride, int heads_box, int rows) {
+  const int64_t dims[3] = {dim, heads, tokens}, strides[3] = {1, head_stride, token_stride};
+  const int box[3] = {64, heads_box, rows};
+  return encode(map, base, 3, dims, strides, box);
+}
+
+int encode_pages(CUtensorMap* map, const void* base, const adb::PrefillParams& p, int64_t dim) {
+  const int64_t page = int64_t(1) << p.page_shift;
+  const int rows = static_cast<int>(page < adb::kTile ? page : adb::kTile);
+  if (p.paged == 1) {
+    const int64_t dims[4] = {dim, page, p.kv_heads, p.num_blocks}, strides[4] = {1, dim, page * dim, p.kv_heads * page * dim};
+    const int box[4] = {64, rows, 1, 1};
+    return encode(map, base, 4, dims, strides, box);
+  }
+  const int64_t dims[4] = {dim, p.kv_heads, page, p.num_blocks}, strides[4] = {1, dim, p.kv_heads * dim, p.kv_heads * page * dim};
+  const int box[4] = {64, 1, rows, 1};
+  return encode(map, base, 4, dims, strides, box);
+}
+
+// The kernel's shared-memory limit is set once per device.
+int prepare(int device) {
+  static std::atomic<uint64_t> done{0};
+  const uint64_t bit = uint64_t(1) << device;
+  if (done.load(std::memory_order_acquire) & bit) return ADB_OK;
+  cudaError_t e = cudaFuncSetAttribute(&adb::prefill_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       adb::PrefillCfg<128>::kSmemBytes);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(&adb::prefill_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             adb::PrefillCfg<64>::kSmemBytes);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(max dynamic smem)");
+  done.fetch_or(bit, std::memory_order_release);
+  return ADB_OK;
+}
+
+// `k`, the K tensor; p holds everything else.
+int launch(adb::PrefillParams& p, const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
+           int64_t k_head, int64_t dim, int device, void* stream) {
   DeviceGuard guard(device);
   if (guard.error != cudaSuccess) return cuda_fail(guard.error, "cudaSetDevice");
   int sms = 0;
-  const int rc = adb_host::sm_count(device, &sms);
+  int rc = adb_host::sm_count(device, &sms);
+  if (rc == ADB_OK) rc = prepare(device);
   if (rc != ADB_OK) return rc;
-  p.scale_log2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(head_dim)));
+  p.scale_log2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(dim)));
+  p.tile_tokens = adb::kTile / p.group;
+  CUtensorMap q_map, k_map, v_map;
+  rc = encode_packed(&q_map, q, p.total, p.q_heads, dim, q_token, q_head, p.group, p.tile_tokens);
+  if (rc != ADB_OK) return rc;
+  if (p.paged) {
+    rc = encode_pages(&k_map, k, p, dim);
+    if (rc == ADB_OK) rc = encode_pages(&v_map, p.v, p, dim);
+  } else {
+    rc = encode_packed(&k_map, k, p.total, p.kv_heads, dim, k_token, k_head, 1, adb::kTile);
+    if (rc == ADB_OK) rc = encode_packed(&v_map, p.v, p.total, p.kv_heads, dim, p.v_token, p.v_head, 1, adb::kTile);
+  }
+  if (rc != ADB_OK) return rc;
+  // every sequence with a token may end in a partly filled pair of tiles
+  const int64_t per = 2 * p.tile_tokens;
+  const int64_t pairs = p.total / per + std::min(p.batch, p.total);
+  if (pairs * p.kv_heads > INT32_MAX) return fail(ADB_ERR_INVALID_ARGUMENT, "too many tiles for one call");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(p.total) * p.q_heads + 3) / 4));
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3(static_cast<unsigned>(pairs * p.kv_heads));
+  cfg.blockDim = dim3(adb::kPrefillThreads);
+  cfg.dynamicSmemBytes = dim == 128 ? adb::PrefillCfg<128>::kSmemBytes : adb::PrefillCfg<64>::kSmemBytes;
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(
-      &cfg, head_dim == 128 ? adb::prefill_rows_kernel<128> : adb::prefill_rows_kernel<64>, p);
+  const cudaError_t e = dim == 128 ? cudaLaunchKernelEx(&cfg, adb::prefill_kernel<128>, q_map, k_map, v_map, p)
+                                   : cudaLaunchKernelEx(&cfg, adb::prefill_kernel<64>, q_map, k_map, v_map, p);
   if (e != cudaSuccess) return cuda_fail(e, "prefill kernel launch");
   adb_host::count_launch();
   return ADB_OK;
@@ -94,13 +172,7 @@ int adb_prefill(const void* q, int64_t q_token_stride, int64_t q_head_stride, co
       ((q_token_stride | q_head_stride | k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7) != 0)
     return fail(ADB_ERR_INVALID_ARGUMENT, "Q, K and V must be 16-byte aligned, their strides multiples of 8 elements");
   adb::PrefillParams p = {};
-  p.q = static_cast<const __nv_bfloat16*>(q);
-  p.k = static_cast<const __nv_bfloat16*>(k);
   p.v = static_cast<const __nv_bfloat16*>(v);
-  p.q_token = q_token_stride;
-  p.q_head = q_head_stride;
-  p.k_token = k_token_stride;
-  p.k_head = k_head_stride;
   p.v_token = v_token_stride;
   p.v_head = v_head_stride;
   p.out = static_cast<__nv_bfloat16*>(out);
@@ -110,7 +182,7 @@ int adb_prefill(const void* q, int64_t q_token_stride, int64_t q_head_stride, co
   p.q_heads = static_cast<int>(q_heads);
   p.kv_heads = static_cast<int>(kv_heads);
   p.group = static_cast<int>(q_heads / kv_heads);
-  return launch(p, head_dim, device, stream);
+  return launch(p, q, q_token_stride, q_head_stride, k, k_token_stride, k_head_stride, head_dim, device, stream);
 }
 
 int adb_prefill_paged(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
@@ -142,11 +214,7 @@ int adb_prefill_paged(const void* q, int64_t q_token_stride, int64_t q_head_stri
       ((q_token_stride | q_head_stride) & 7) != 0)
     return fail(ADB_ERR_INVALID_ARGUMENT, "Q and caches must be 16-byte aligned, Q's strides multiples of 8 elements");
   adb::PrefillParams p = {};
-  p.q = static_cast<const __nv_bfloat16*>(q);
-  p.k = static_cast<const __nv_bfloat16*>(k_cache);
   p.v = static_cast<const __nv_bfloat16*>(v_cache);
-  p.q_token = q_token_stride;
-  p.q_head = q_head_stride;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.cu = cu_seqlens;
   p.lens = seqlens;
@@ -161,7 +229,7 @@ int adb_prefill_paged(const void* q, int64_t q_token_stride, int64_t q_head_stri
   p.max_blocks = static_cast<int>(max_blocks_per_seq);
   p.num_blocks = static_cast<int>(num_blocks);
   while ((int64_t(1) << p.page_shift) < page_size) ++p.page_shift;
-  return launch(p, head_dim, device, stream);
+  return launch(p, q, q_token_stride, q_head_stride, k_cache, 0, 0, head_dim, device, stream);
 }
 
 }  // extern "C"

@@ -5,87 +5,513 @@
 // c_b = L_b - n_b tokens come before the n_b new ones (0 for packed prompts):
 //     o = sum_{j <= p} softmax_j(q . k_j / sqrt(D)) v_j,   h_kv = h / G
 // with an FP32 online softmax.  A row that sees no key is zero.
+//
+// Rows.  The G query heads that share a KV head are packed into the 128 rows
+// of a tensor-core tile beside 128 / G consecutive tokens (row = token * G +
+// head), so that every K/V tile serves all of them and short chunks still
+// fill tiles; any G up to 64 works.  A CTA owns two such tiles of one
+// (sequence, KV head) and streams the K/V tiles (128 keys) that they see.
+//
+// Pipeline of a CTA (384 threads):
+//   warps 0-3, 4-7   softmax of tile 0, 1: one thread per row
+//   warp 8           TMA loads: Q once, then K_0 V_0 K_1 V_1 ... into a ring
+//   warp 9           issues the tensor-core products (one thread)
+//   warp 10          clears masked V rows of border tiles (below)
+// S_i = Q_i K_j^T (FP32) and O_i live in tensor memory; the softmax thread
+// reads its row of S_i, writes the weights P_i (BF16) over it, and the product
+// O_i += P_i V_j takes P_i from tensor memory.  While one tile's softmax runs
+// the tensor cores work on the other tile.
+//
+// The running maximum is raised (and O rescaled) only when it grows by more
+// than 2^8: until then weights up to 2^8 are exact enough in FP32 sums and in
+// BF16's relative rounding, and the factor cancels in O / l.
+//
+// Masked keys have weight 0, and 0 * NaN is NaN: rows of V behind the sequence
+// (recycled pages, the next sequence) are therefore cleared in shared memory,
+// and non-finite values of V that only some rows of the tiles may see are
+// cleared there and added to those rows at the end.
 #pragma once
 
-#include "device_primitives.cuh"
+#include "tcgen05_primitives.cuh"
 
 namespace adb {
 
+constexpr int kPrefillThreads = 384;
+constexpr int kTile = 128;  // rows of a Q tile, keys of a K/V tile
+constexpr float kRescaleLog2 = 8.f;
+
 struct PrefillParams {
-  const __nv_bfloat16* q;  // [total][q_heads][D], strides in elements
-  const __nv_bfloat16* k;  // [total][kv_heads][D], or the pool of pages
-  const __nv_bfloat16* v;
-  int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+  const __nv_bfloat16* v;  // [total][kv_heads][D] or the pool of pages (non-finite values only)
+  int64_t v_token, v_head;
   __nv_bfloat16* out;      // [total][q_heads][D], contiguous
   const int32_t* cu;       // [batch + 1]
   const int32_t* lens;     // [batch] tokens in the cache, new ones included (paged)
   const int32_t* table;    // paged: [batch][max_blocks]
   int64_t table_stride;
   int total, batch, q_heads, kv_heads, group;
+  int tile_tokens;         // tokens of a Q tile: 128 / group
   int paged;               // 0 packed K/V, 1 HND pages, 2 NHD pages
   int max_blocks, num_blocks, page_shift;
   float scale_log2;        // log2(e) / sqrt(D)
 };
 
-// One warp per row: the lanes share the head dimension.
 template <int D>
-__global__ void __launch_bounds__(128) prefill_rows_kernel(const PrefillParams p) {
-  constexpr int E = D / 32;
+struct PrefillCfg {
+  static constexpr int kHalves = D / 64;                     // 128-byte column blocks of a row
+  static constexpr int kHalfBytes = kTile * 128;             // one column block of a tile
+  static constexpr int kTileBytes = kHalves * kHalfBytes;
+  static constexpr int kStages = D == 128 ? 5 : 8;           // K and V tiles in flight
+  static constexpr int kVPeriod = kStages % 2 ? kStages : kStages / 2;  // V tiles until a stage holds V again
+  static constexpr int kSmemBytes = (2 + kStages) * kTileBytes + 1024;
+};
+
+// What a CTA works on.
+struct PrefillWork {
+  int seq, head;     // sequence, KV head (seq < 0: nothing)
+  int row0;          // first row of the sequence in q / out
+  int token0;        // first token of tile 0, within the sequence's new ones
+  int tokens;        // new tokens of the sequence
+  int before;        // keys before token 0 (may be negative)
+  int keys;          // keys of the sequence
+};
+
+template <int D>
+struct PrefillShared {
+  alignas(8) uint64_t q_full;
+  uint64_t kv_full[PrefillCfg<D>::kStages], kv_empty[PrefillCfg<D>::kStages];
+  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t v_turn[PrefillCfg<D>::kStages];   // a border tile of V is on its way
+  uint64_t v_clean[PrefillCfg<D>::kStages];  // and cleared
+  uint64_t fix_done;
+  uint32_t tmem;
+  int abort;
+  int fix;           // a non-finite value of V was cleared
+  PrefillWork work;
+};
+
+__device__ __forceinline__ int clamp_to(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }
+
+// First row and row count of sequence b, whatever cu holds.
+__device__ __forceinline__ void sequence_rows(const PrefillParams& p, int b, int& first, int& count) {
+  first = clamp_to(p.cu[b], 0, p.total);
+  count = clamp_to(p.cu[b + 1], first, p.total) - first;
+}
+
+// The item-th pair of tiles over all sequences (one warp; the result is the
+// same in all lanes).
+__device__ __forceinline__ void find_work(const PrefillParams& p, int index, PrefillWork& w) {
   const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  griddep_wait();
-  if (row >= static_cast<int64_t>(p.total) * p.q_heads) return;
-  const int t = static_cast<int>(row / p.q_heads), h = static_cast<int>(row % p.q_heads), hkv = h / p.group;
-  int lo = 0, hi = p.batch - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (p.cu[mid] <= t)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  const int first = p.cu[lo], last = min(p.cu[lo + 1], p.total);
-  int keys = 0;
-  if (t >= first && t < last) {
-    const int cap = p.paged ? p.max_blocks << p.page_shift : 0;
-    const int len = p.paged ? min(max(p.lens[lo], 0), cap) : last - first;
-    keys = max(0, len - (last - first) + (t - first) + 1);
-  }
-  float q[E], acc[E] = {};
-  for (int e = 0; e < E; ++e)
-    q[e] = __bfloat162float(p.q[t * p.q_token + h * p.q_head + lane * E + e]) * p.scale_log2;
-  float m = -INFINITY, l = 0.f;
-  for (int j = 0; j < keys; ++j) {
-    int64_t ka, va;
-    if (p.paged) {
-      const int page = p.table[lo * p.table_stride + (j >> p.page_shift)];
-      if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_blocks)) {  // counts as zeros
-        if (lane == 0) atomicOr(&g_adb_error_flag, kErrCachePage);
-        const float top = fmaxf(m, 0.f), keep = m == top ? 1.f : exp2f(m - top);
-        m = top;
-        l = l * keep + exp2f(-top);
-        for (int e = 0; e < E; ++e) acc[e] *= keep;
-        continue;
-      }
-      const int64_t size = int64_t(1) << p.page_shift, slot = j & (size - 1);
-      ka = (p.paged == 1 ? (static_cast<int64_t>(page) * p.kv_heads + hkv) * size + slot
-                         : (page * size + slot) * p.kv_heads + hkv) * D;
-      va = ka;
-    } else {
-      ka = static_cast<int64_t>(first + j) * p.k_token + hkv * p.k_head;
-      va = static_cast<int64_t>(first + j) * p.v_token + hkv * p.v_head;
+  const int item = index / p.kv_heads;
+  const int per = 2 * p.tile_tokens;
+  w.head = index - item * p.kv_heads;
+  w.seq = -1;
+  int before = 0;
+  for (int base = 0; base < p.batch; base += 32) {
+    int first = 0, count = 0;
+    if (base + lane < p.batch) sequence_rows(p, base + lane, first, count);
+    const int mine = (count + per - 1) / per;
+    int inc = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, inc, d);
+      if (lane >= d) inc += o;
     }
-    float s = 0.f;
-    for (int e = 0; e < E; ++e) s += q[e] * __bfloat162float(p.k[ka + lane * E + e]);
-    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    const float top = fmaxf(m, s);
-    const float keep = m == top ? 1.f : exp2f(m - top), w = exp2f(s - top);
-    m = top;
-    l = l * keep + w;
-    for (int e = 0; e < E; ++e) acc[e] = acc[e] * keep + w * __bfloat162float(p.v[va + lane * E + e]);
+    const unsigned hit = __ballot_sync(0xffffffffu, item < before + inc);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      w.seq = base + l;
+      w.row0 = __shfl_sync(0xffffffffu, first, l);
+      w.tokens = __shfl_sync(0xffffffffu, count, l);
+      const int items = __shfl_sync(0xffffffffu, mine, l);
+      const int at = item - before - (__shfl_sync(0xffffffffu, inc, l) - items);
+      w.token0 = (items - 1 - at) * per;  // the pair that sees the most keys first
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, inc, 31);
   }
-  for (int e = 0; e < E; ++e)
-    p.out[row * D + lane * E + e] = __float2bfloat16(keys > 0 ? acc[e] / l : 0.f);
+  if (w.seq < 0) return;
+  w.keys = w.tokens;
+  if (p.paged) w.keys = clamp_to(p.lens[w.seq], 0, p.max_blocks << p.page_shift);
+  w.before = w.keys - w.tokens;
+}
+
+// Keys that token t of the work's sequence sees (0 or less: none).
+__device__ __forceinline__ int keys_of(const PrefillWork& w, int t) { return w.before + t + 1; }
+
+// Valid tokens of tile i and the K/V tiles that it needs.
+__device__ __forceinline__ int tile_valid(const PrefillParams& p, const PrefillWork& w, int i) {
+  return clamp_to(w.tokens - w.token0 - i * p.tile_tokens, 0, p.tile_tokens);
+}
+__device__ __forceinline__ int tile_steps(const PrefillParams& p, const PrefillWork& w, int i) {
+  const int valid = tile_valid(p, w, i);
+  const int last = keys_of(w, w.token0 + i * p.tile_tokens + valid - 1);
+  return valid > 0 && last > 0 ? (last + kTile - 1) / kTile : 0;
+}
+
+// A wait of a whole warp, with one answer for all lanes.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, abort));
+}
+
+// Sum of the non-finite values of V[key][d], key in [lo, hi): what the cleared
+// values add to a row that sees them.
+__device__ __noinline__ float non_finite_sum(const PrefillParams& p, int seq, int head, int row0, int dim, int lo,
+                                             int hi, int d) {
+  float sum = 0.f;
+  for (int key = max(lo, 0); key < hi; ++key) {
+    int64_t at;
+    if (p.paged) {
+      const int page = p.table[seq * p.table_stride + (key >> p.page_shift)];
+      if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_blocks)) continue;
+      const int64_t size = int64_t(1) << p.page_shift, slot = key & (size - 1);
+      at = (p.paged == 1 ? (static_cast<int64_t>(page) * p.kv_heads + head) * size + slot
+                         : (page * size + slot) * p.kv_heads + head) * dim;
+    } else {
+      at = static_cast<int64_t>(row0 + key) * p.v_token + head * p.v_head;
+    }
+    const float x = __bfloat162float(p.v[at + d]);
+    if (!(fabsf(x) <= 3.4e38f)) sum += x;
+  }
+  return sum;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kPrefillThreads, 1)
+    prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                   const __grid_constant__ CUtensorMap v_map, const __grid_constant__ PrefillParams p) {
+  using C = PrefillCfg<D>;
+  extern __shared__ uint8_t raw[];
+  __shared__ PrefillShared<D> sh;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const uint32_t tiles = (smem_u32(raw) + 1023u) & ~1023u;  // Q_0 Q_1, then the K/V ring
+  const uint32_t ring = tiles + 2 * C::kTileBytes;
+  volatile int* abort = &sh.abort;
+
+  if (tid == 0) {
+    mbar_init(smem_u32(&sh.q_full), 1);
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(smem_u32(&sh.kv_full[s]), 1);
+      mbar_init(smem_u32(&sh.kv_empty[s]), 1);
+      mbar_init(smem_u32(&sh.v_turn[s]), 1);
+      mbar_init(smem_u32(&sh.v_clean[s]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&sh.s_full[i]), 1);
+      mbar_init(smem_u32(&sh.p_full[i]), 4);
+      mbar_init(smem_u32(&sh.o_full[i]), 1);
+    }
+    mbar_init(smem_u32(&sh.fix_done), 1);
+    sh.abort = 0;
+    sh.fix = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) tmem_alloc(smem_u32(&sh.tmem), 512);
+  griddep_wait();
+  if (warp == 8) {
+    PrefillWork w;
+    find_work(p, blockIdx.x, w);
+    if (lane == 0) sh.work = w;
+  }
+  // padding: rows before the first and behind the last sequence
+  {
+    const int from = clamp_to(p.cu[p.batch], 0, p.total), head = clamp_to(p.cu[0], 0, p.total);
+    const int64_t vecs = static_cast<int64_t>(p.q_heads) * (D / 8);
+    uint4* o = reinterpret_cast<uint4*>(p.out);
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kPrefillThreads;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * kPrefillThreads + tid;
+    for (int64_t i = from * vecs + at; i < p.total * vecs; i += step) o[i] = make_uint4(0, 0, 0, 0);
+    for (int64_t i = at; i < head * vecs; i += step) o[i] = make_uint4(0, 0, 0, 0);
+  }
+  tcgen05_before_sync();
+  __syncthreads();
+  tcgen05_after_sync();
+  const PrefillWork w = sh.work;
+  const uint32_t tmem = sh.tmem;
+  const int steps0 = w.seq < 0 ? 0 : tile_steps(p, w, 0), steps1 = w.seq < 0 ? 0 : tile_steps(p, w, 1);
+  const int steps = max(steps0, steps1);
+  // keys from here on are hidden from some row of the tiles
+  const int open_keys = w.seq < 0 ? 0 : max(keys_of(w, w.token0), 0);
+
+  if (warp == 8) {
+    // ------------------------------------------------------------ loads
+    if (steps > 0) {
+      const int boxes = p.paged ? max(1, kTile >> p.page_shift) : 1;
+      const int box_rows = kTile / boxes;
+      if (lane == 0) {
+        const uint32_t bar = smem_u32(&sh.q_full);
+        const int n = steps1 > 0 ? 2 : 1;
+        mbar_arrive_expect_tx(bar, n * C::kHalves * p.tile_tokens * p.group * 128);
+        for (int i = 0; i < n; ++i)
+          for (int h = 0; h < C::kHalves; ++h)
+            tma_load_tile_3d(tiles + i * C::kTileBytes + h * C::kHalfBytes, &q_map, h * 64, w.head * p.group,
+                              w.row0 + w.token0 + i * p.tile_tokens, bar);
+      }
+      for (int t = 0; t < 2 * steps; ++t) {
+        const int stage = t % C::kStages;
+        if (t >= C::kStages) {
+          if (!warp_wait(&sh.kv_empty[stage], (t / C::kStages - 1) & 1, abort)) break;
+        }
+        const int key0 = (t >> 1) * kTile;
+        const uint32_t bar = smem_u32(&sh.kv_full[stage]);
+        const CUtensorMap* map = (t & 1) ? &v_map : &k_map;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(bar, C::kTileBytes);
+          if ((t & 1) && (t >> 1) >= open_keys / kTile) mbar_arrive(smem_u32(&sh.v_turn[stage]));
+        }
+        __syncwarp();
+        if (lane < boxes) {
+          const int key = key0 + lane * box_rows;
+          const uint32_t dst = ring + stage * C::kTileBytes + lane * box_rows * 128;
+          int page = -1;  // outside the pool: reads as zeros
+          if (p.paged && key < w.keys) {
+            page = p.table[w.seq * p.table_stride + (key >> p.page_shift)];
+            if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_blocks)) {
+              page = -1;
+              atomicOr(&g_adb_error_flag, kErrCachePage);
+            }
+          }
+          const int slot = key & ((1 << p.page_shift) - 1);
+          for (int h = 0; h < C::kHalves; ++h) {
+            if (!p.paged)
+              tma_load_tile_3d(dst + h * C::kHalfBytes, map, h * 64, w.head, w.row0 + key, bar);
+            else if (p.paged == 1)
+              tma_load_tile_4d(dst + h * C::kHalfBytes, map, h * 64, slot, w.head, page, bar);
+            else
+              tma_load_tile_4d(dst + h * C::kHalfBytes, map, h * 64, w.head, slot, page, bar);
+          }
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------------ products
+    if (lane == 0 && steps > 0) {
+      constexpr uint64_t k_major = smem_desc_base(16, 1024);
+      constexpr uint64_t v_major = smem_desc_base(C::kHalfBytes, 1024);
+      constexpr uint32_t qk_idesc = mma_idesc(kTile, kTile, false);
+      constexpr uint32_t pv_idesc = mma_idesc(kTile, D, true);
+      const auto qk = [&](int i, int stage) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t at = (k >> 2) * C::kHalfBytes + (k & 3) * 32;
+          mma_ss(tmem + i * kTile, smem_desc(k_major, tiles + i * C::kTileBytes + at),
+                 smem_desc(k_major, ring + stage * C::kTileBytes + at), qk_idesc, k > 0);
+        }
+        mma_commit(smem_u32(&sh.s_full[i]));
+      };
+      const auto full = [&](int t) {
+        return mbar_wait(smem_u32(&sh.kv_full[t % C::kStages]), (t / C::kStages) & 1, abort);
+      };
+      bool ok = mbar_wait(smem_u32(&sh.q_full), 0, abort) && full(0);
+      if (ok) {
+        tcgen05_after_sync();
+        if (steps0 > 0) qk(0, 0);
+        if (steps1 > 0) qk(1, 0);
+        if (C::kStages < 2 * steps) mma_commit(smem_u32(&sh.kv_empty[0]));
+      }
+      const int first_open = open_keys / kTile;
+      for (int j = 0; ok && j < steps; ++j) {
+        const int tv = 2 * j + 1, tk = 2 * j + 2;
+        bool v_ready = false, k_ready = false;
+        for (int i = 0; ok && i < 2; ++i) {
+          const int mine = i ? steps1 : steps0;
+          if (j >= mine) continue;
+          if (!v_ready) {
+            ok = full(tv);
+            if (ok && j >= first_open)
+              ok = mbar_wait(smem_u32(&sh.v_clean[tv % C::kStages]), ((j - first_open) / C::kVPeriod) & 1, abort);
+            v_ready = true;
+          }
+          if (ok) ok = mbar_wait(smem_u32(&sh.p_full[i]), j & 1, abort);
+          if (!ok) break;
+          tcgen05_after_sync();
+#pragma unroll
+          for (int k = 0; k < kTile / 16; ++k)
+            mma_ts(tmem + 2 * kTile + i * kTile, tmem + i * kTile + k * 8,
+                   smem_desc(v_major, ring + (tv % C::kStages) * C::kTileBytes + k * 2048), pv_idesc, j > 0 || k > 0);
+          if (j + 1 == mine) {
+            mma_commit(smem_u32(&sh.o_full[i]));
+          } else {
+            if (!k_ready) ok = full(tk);
+            k_ready = true;
+            if (ok) qk(i, tk % C::kStages);
+          }
+        }
+        if (ok) {
+          // (no arrival that nobody waits for: it could come after the CTA is gone)
+          if (tv + C::kStages < 2 * steps) mma_commit(smem_u32(&sh.kv_empty[tv % C::kStages]));
+          if (tk + C::kStages < 2 * steps) mma_commit(smem_u32(&sh.kv_empty[tk % C::kStages]));
+        }
+      }
+    }
+  } else if (warp == 10) {
+    // ------------------------------------------------------------ masked V
+    bool fix = false;
+    for (int j = open_keys / kTile; j < steps; ++j) {
+      const int t = 2 * j + 1;
+      // the loads' word that the stage has come to tile t, whose parity then is unmistakable
+      if (!warp_wait(&sh.v_turn[t % C::kStages], ((j - open_keys / kTile) / C::kVPeriod) & 1, abort)) break;
+      if (!warp_wait(&sh.kv_full[t % C::kStages], (t / C::kStages) & 1, abort)) break;
+      const int first = max(open_keys - j * kTile, 0);      // first key that some row may not see
+      const int behind = clamp_to(w.keys - j * kTile, 0, kTile);  // first key behind the sequence
+      for (int h = 0; h < C::kHalves; ++h) {
+        const uint32_t base = ring + (t % C::kStages) * C::kTileBytes + h * C::kHalfBytes;
+        for (int x = first * 8 + lane; x < kTile * 8; x += 32) {
+          const uint32_t at = base + x * 16;
+          uint32_t v[4] = {0, 0, 0, 0};
+          bool write = x >= behind * 8;
+          if (!write) {
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                         : "r"(at));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              // exponent all ones: infinite or not a number
+              if ((v[e] & 0x7F80u) == 0x7F80u) v[e] &= 0xFFFF0000u, write = fix = true;
+              if ((v[e] & 0x7F800000u) == 0x7F800000u) v[e] &= 0xFFFFu, write = fix = true;
+            }
+          }
+          if (write)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                         "r"(v[3])
+                         : "memory");
+        }
+      }
+      fence_proxy_async_shared();
+      fix = __any_sync(0xffffffffu, fix);
+      if (lane == 0) mbar_arrive(smem_u32(&sh.v_clean[t % C::kStages]));
+      __syncwarp();
+    }
+    if (lane == 0) {
+      if (fix) *reinterpret_cast<volatile int*>(&sh.fix) = 1;
+      mbar_arrive(smem_u32(&sh.fix_done));
+    }
+  } else if (warp < 8) {
+    // ------------------------------------------------------------ softmax
+    const int i = warp >> 2;
+    const int mine = i ? steps1 : steps0;
+    const int row = tid & (kTile - 1);
+    const int valid = w.seq < 0 ? 0 : tile_valid(p, w, i);
+    const int token = row / p.group;
+    const bool live = row < p.tile_tokens * p.group && token < valid;
+    const int t = w.token0 + i * p.tile_tokens + token;
+    const int sees = live ? keys_of(w, t) : 0;
+    const int all_see = keys_of(w, w.token0 + i * p.tile_tokens);  // keys that every row of the tile sees
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + i * kTile + lanes, o_at = tmem + 2 * kTile + i * kTile + lanes;
+    const float scale = p.scale_log2;
+    float top = -INFINITY, total = 0.f;
+    bool ok = true;
+    for (int j = 0; j < mine; ++j) {
+      ok = warp_wait(&sh.s_full[i], j & 1, abort);
+      if (!ok) break;
+      tcgen05_after_sync();
+      float s[kTile];
+#pragma unroll
+      for (int c = 0; c < kTile; c += 32) tmem_ld32(s_at + c, s + c);
+      tmem_wait_ld();
+      if ((j + 1) * kTile > all_see) {
+        const int limit = sees - j * kTile;
+#pragma unroll
+        for (int c = 0; c < kTile; ++c) s[c] = c < limit ? s[c] : -INFINITY;
+      }
+      float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
+#pragma unroll
+      for (int c = 4; c < kTile; c += 4) {
+        m0 = fmaxf(m0, s[c]);
+        m1 = fmaxf(m1, s[c + 1]);
+        m2 = fmaxf(m2, s[c + 2]);
+        m3 = fmaxf(m3, s[c + 3]);
+      }
+      const float high = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+      if (j == 0) {
+        top = high;
+      } else if (__any_sync(0xffffffffu, live && (high - top) * scale > kRescaleLog2)) {
+        // O_i holds the sum up to tile j - 1: S_i was issued after that product.  Rows outside the
+        // sequence have no say: the result would depend on what lies there.
+        const float next = fmaxf(top, high);
+        const float keep = next == top ? 1.f : fast_exp2((top - next) * scale);
+        top = next;
+        total *= keep;
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          float o[32];
+          tmem_ld32(o_at + c, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] *= keep;
+          tmem_st32(o_at + c, o);
+        }
+      }
+      const float shift = top == -INFINITY ? 0.f : -top * scale;
+      const uint64_t scale2 = pack2(scale, scale), shift2 = pack2(shift, shift);
+      uint64_t sum0 = 0, sum1 = 0;
+#pragma unroll
+      for (int c = 0; c < kTile; c += 32) {
+        uint32_t w16[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float a, b;
+          unpack2(fma2(pack2(s[c + 2 * e], s[c + 2 * e + 1]), scale2, shift2), a, b);
+          a = fast_exp2(a);
+          b = fast_exp2(b);
+          if (e & 1)
+            sum1 = add2(sum1, pack2(a, b));
+          else
+            sum0 = add2(sum0, pack2(a, b));
+          w16[e] = pack_bf16x2(a, b);
+        }
+        tmem_st16(s_at + c / 2, w16);
+      }
+      tmem_wait_st();
+      tcgen05_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[i]));
+      float a, b;
+      unpack2(add2(sum0, sum1), a, b);
+      total += a + b;
+    }
+    if (mine > 0 && ok) {
+      ok = warp_wait(&sh.fix_done, 0, abort) && warp_wait(&sh.o_full[i], 0, abort);
+      tcgen05_after_sync();
+    }
+    const bool fix = *reinterpret_cast<volatile int*>(&sh.fix) != 0;
+    const float inv = mine == 0 || total == 0.f ? 0.f : 1.f / total;
+    __nv_bfloat16* out = p.out + (static_cast<int64_t>(w.row0 + t) * p.q_heads + w.head * p.group + row % p.group) * D;
+    if (ok && valid > 0) {
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        float o[32];
+        if (mine > 0) {
+          tmem_ld32(o_at + c, o);
+          tmem_wait_ld();
+        }
+        uint32_t x[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float a = inv == 0.f ? 0.f : o[2 * e] * inv, b = inv == 0.f ? 0.f : o[2 * e + 1] * inv;
+          if (fix && live) {
+            a += non_finite_sum(p, w.seq, w.head, w.row0, D, open_keys, sees, c + 2 * e);
+            b += non_finite_sum(p, w.seq, w.head, w.row0, D, open_keys, sees, c + 2 * e + 1);
+          }
+          x[e] = pack_bf16x2(a, b);
+        }
+        if (live) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<uint4*>(out + c + e * 8) = make_uint4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+        }
+      }
+    }
+    tcgen05_before_sync();
+  }
+  __syncthreads();
+  griddep_launch_dependents();
+  if (warp == 9) {
+    tcgen05_after_sync();
+    tmem_dealloc(tmem, 512);
+  }
 }
 
 }  // namespace adb
