@@ -97,6 +97,15 @@ int prepare(int device) {
     e = cudaFuncSetAttribute(&adb::prefill_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              adb::PrefillCfg<64>::kSmemBytes);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(max dynamic smem)");
+  // The warps' register split counts on what the block is launched with.
+  for (const void* fn : {reinterpret_cast<const void*>(&adb::prefill_kernel<128>),
+                         reinterpret_cast<const void*>(&adb::prefill_kernel<64>)}) {
+    cudaFuncAttributes a;
+    e = cudaFuncGetAttributes(&a, fn);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncGetAttributes");
+    if (a.numRegs * 3 < 2 * adb::kSoftmaxRegs + adb::kOtherRegs)
+      return fail(ADB_ERR_CUDA, "the prefill kernel was compiled to %d registers, too few for its split", a.numRegs);
+  }
   done.fetch_or(bit, std::memory_order_release);
   return ADB_OK;
 }

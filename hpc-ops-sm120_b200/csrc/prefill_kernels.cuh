@@ -38,7 +38,11 @@ namespace adb {
 
 constexpr int kPrefillThreads = 384;
 constexpr int kTile = 128;  // rows of a Q tile, keys of a K/V tile
+constexpr int kFirstPart = 64;  // keys whose weights are handed to the tensor cores before the others are computed
 constexpr float kRescaleLog2 = 8.f;
+// Registers: 12 warps x 168 at launch; the loading and issuing warps give theirs to the softmax.
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
+static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * 168, "more registers than the block is launched with");
 
 struct PrefillParams {
   const __nv_bfloat16* v;  // [total][kv_heads][D] or the pool of pages (non-finite values only)
@@ -79,7 +83,7 @@ template <int D>
 struct PrefillShared {
   alignas(8) uint64_t q_full;
   uint64_t kv_full[PrefillCfg<D>::kStages], kv_empty[PrefillCfg<D>::kStages];
-  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t s_full[2], p_part[2], p_full[2], o_full[2];
   uint64_t v_turn[PrefillCfg<D>::kStages];   // a border tile of V is on its way
   uint64_t v_clean[PrefillCfg<D>::kStages];  // and cleared
   uint64_t fix_done;
@@ -153,11 +157,10 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, abort));
 }
 
-// Sum of the non-finite values of V[key][d], key in [lo, hi): what the cleared
-// values add to a row that sees them.
-__device__ __noinline__ float non_finite_sum(const PrefillParams& p, int seq, int head, int row0, int dim, int lo,
-                                             int hi, int d) {
-  float sum = 0.f;
+// Adds the non-finite values of V[key][d], key in [lo, hi), that were cleared
+// for the tile to the row `out` that sees them.
+__device__ __noinline__ void add_non_finite(const PrefillParams& p, int seq, int head, int row0, int dim, int lo,
+                                            int hi, __nv_bfloat16* out) {
   for (int key = max(lo, 0); key < hi; ++key) {
     int64_t at;
     if (p.paged) {
@@ -169,10 +172,11 @@ __device__ __noinline__ float non_finite_sum(const PrefillParams& p, int seq, in
     } else {
       at = static_cast<int64_t>(row0 + key) * p.v_token + head * p.v_head;
     }
-    const float x = __bfloat162float(p.v[at + d]);
-    if (!(fabsf(x) <= 3.4e38f)) sum += x;
+    for (int d = 0; d < dim; ++d) {
+      const float x = __bfloat162float(p.v[at + d]);
+      if (!(fabsf(x) <= 3.4e38f)) out[d] = __float2bfloat16(__bfloat162float(out[d]) + x);
+    }
   }
-  return sum;
 }
 
 template <int D>
@@ -198,6 +202,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&sh.s_full[i]), 1);
+      mbar_init(smem_u32(&sh.p_part[i]), 4);
       mbar_init(smem_u32(&sh.p_full[i]), 4);
       mbar_init(smem_u32(&sh.o_full[i]), 1);
     }
@@ -233,162 +238,176 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   // keys from here on are hidden from some row of the tiles
   const int open_keys = w.seq < 0 ? 0 : max(keys_of(w, w.token0), 0);
 
-  if (warp == 8) {
-    // ------------------------------------------------------------ loads
-    if (steps > 0) {
-      const int boxes = p.paged ? max(1, kTile >> p.page_shift) : 1;
-      const int box_rows = kTile / boxes;
-      if (lane == 0) {
-        const uint32_t bar = smem_u32(&sh.q_full);
-        const int n = steps1 > 0 ? 2 : 1;
-        mbar_arrive_expect_tx(bar, n * C::kHalves * p.tile_tokens * p.group * 128);
-        for (int i = 0; i < n; ++i)
-          for (int h = 0; h < C::kHalves; ++h)
-            tma_load_tile_3d(tiles + i * C::kTileBytes + h * C::kHalfBytes, &q_map, h * 64, w.head * p.group,
-                              w.row0 + w.token0 + i * p.tile_tokens, bar);
-      }
-      for (int t = 0; t < 2 * steps; ++t) {
-        const int stage = t % C::kStages;
-        if (t >= C::kStages) {
-          if (!warp_wait(&sh.kv_empty[stage], (t / C::kStages - 1) & 1, abort)) break;
-        }
-        const int key0 = (t >> 1) * kTile;
-        const uint32_t bar = smem_u32(&sh.kv_full[stage]);
-        const CUtensorMap* map = (t & 1) ? &v_map : &k_map;
+  if (warp >= 8) {
+    regs_dec<kOtherRegs>();
+    if (warp == 8) {
+      // ------------------------------------------------------------ loads
+      if (steps > 0) {
+        const int boxes = p.paged ? max(1, kTile >> p.page_shift) : 1;
+        const int box_rows = kTile / boxes;
         if (lane == 0) {
-          mbar_arrive_expect_tx(bar, C::kTileBytes);
-          if ((t & 1) && (t >> 1) >= open_keys / kTile) mbar_arrive(smem_u32(&sh.v_turn[stage]));
+          const uint32_t bar = smem_u32(&sh.q_full);
+          const int n = steps1 > 0 ? 2 : 1;
+          mbar_arrive_expect_tx(bar, n * C::kHalves * p.tile_tokens * p.group * 128);
+          for (int i = 0; i < n; ++i)
+            for (int h = 0; h < C::kHalves; ++h)
+              tma_load_tile_3d(tiles + i * C::kTileBytes + h * C::kHalfBytes, &q_map, h * 64, w.head * p.group,
+                                w.row0 + w.token0 + i * p.tile_tokens, bar);
         }
-        __syncwarp();
-        if (lane < boxes) {
-          const int key = key0 + lane * box_rows;
-          const uint32_t dst = ring + stage * C::kTileBytes + lane * box_rows * 128;
-          int page = -1;  // outside the pool: reads as zeros
-          if (p.paged && key < w.keys) {
-            page = p.table[w.seq * p.table_stride + (key >> p.page_shift)];
-            if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_blocks)) {
-              page = -1;
-              atomicOr(&g_adb_error_flag, kErrCachePage);
+        for (int t = 0; t < 2 * steps; ++t) {
+          const int stage = t % C::kStages;
+          if (t >= C::kStages) {
+            if (!warp_wait(&sh.kv_empty[stage], (t / C::kStages - 1) & 1, abort)) break;
+          }
+          const int key0 = (t >> 1) * kTile;
+          const uint32_t bar = smem_u32(&sh.kv_full[stage]);
+          const CUtensorMap* map = (t & 1) ? &v_map : &k_map;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(bar, C::kTileBytes);
+            if ((t & 1) && (t >> 1) >= open_keys / kTile) mbar_arrive(smem_u32(&sh.v_turn[stage]));
+          }
+          __syncwarp();
+          if (lane < boxes) {
+            const int key = key0 + lane * box_rows;
+            const uint32_t dst = ring + stage * C::kTileBytes + lane * box_rows * 128;
+            int page = -1;  // outside the pool: reads as zeros
+            if (p.paged && key < w.keys) {
+              page = p.table[w.seq * p.table_stride + (key >> p.page_shift)];
+              if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_blocks)) {
+                page = -1;
+                atomicOr(&g_adb_error_flag, kErrCachePage);
+              }
+            }
+            const int slot = key & ((1 << p.page_shift) - 1);
+            for (int h = 0; h < C::kHalves; ++h) {
+              if (!p.paged)
+                tma_load_tile_3d(dst + h * C::kHalfBytes, map, h * 64, w.head, w.row0 + key, bar);
+              else if (p.paged == 1)
+                tma_load_tile_4d(dst + h * C::kHalfBytes, map, h * 64, slot, w.head, page, bar);
+              else
+                tma_load_tile_4d(dst + h * C::kHalfBytes, map, h * 64, w.head, slot, page, bar);
             }
           }
-          const int slot = key & ((1 << p.page_shift) - 1);
-          for (int h = 0; h < C::kHalves; ++h) {
-            if (!p.paged)
-              tma_load_tile_3d(dst + h * C::kHalfBytes, map, h * 64, w.head, w.row0 + key, bar);
-            else if (p.paged == 1)
-              tma_load_tile_4d(dst + h * C::kHalfBytes, map, h * 64, slot, w.head, page, bar);
-            else
-              tma_load_tile_4d(dst + h * C::kHalfBytes, map, h * 64, w.head, slot, page, bar);
-          }
+          __syncwarp();
         }
-        __syncwarp();
       }
-    }
-  } else if (warp == 9) {
-    // ------------------------------------------------------------ products
-    if (lane == 0 && steps > 0) {
-      constexpr uint64_t k_major = smem_desc_base(16, 1024);
-      constexpr uint64_t v_major = smem_desc_base(C::kHalfBytes, 1024);
-      constexpr uint32_t qk_idesc = mma_idesc(kTile, kTile, false);
-      constexpr uint32_t pv_idesc = mma_idesc(kTile, D, true);
-      const auto qk = [&](int i, int stage) {
+    } else if (warp == 9) {
+      // ------------------------------------------------------------ products
+      if (lane == 0 && steps > 0) {
+        constexpr uint64_t k_major = smem_desc_base(16, 1024);
+        constexpr uint64_t v_major = smem_desc_base(C::kHalfBytes, 1024);
+        constexpr uint32_t qk_idesc = mma_idesc(kTile, kTile, false);
+        constexpr uint32_t pv_idesc = mma_idesc(kTile, D, true);
+        const auto qk = [&](int i, int stage) {
+          uint64_t a = smem_desc(k_major, tiles + i * C::kTileBytes), b = smem_desc(k_major, ring + stage * C::kTileBytes);
+          keep_here(a);
+          keep_here(b);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t at = (k >> 2) * C::kHalfBytes + (k & 3) * 32;
-          mma_ss(tmem + i * kTile, smem_desc(k_major, tiles + i * C::kTileBytes + at),
-                 smem_desc(k_major, ring + stage * C::kTileBytes + at), qk_idesc, k > 0);
-        }
-        mma_commit(smem_u32(&sh.s_full[i]));
-      };
-      const auto full = [&](int t) {
-        return mbar_wait(smem_u32(&sh.kv_full[t % C::kStages]), (t / C::kStages) & 1, abort);
-      };
-      bool ok = mbar_wait(smem_u32(&sh.q_full), 0, abort) && full(0);
-      if (ok) {
-        tcgen05_after_sync();
-        if (steps0 > 0) qk(0, 0);
-        if (steps1 > 0) qk(1, 0);
-        if (C::kStages < 2 * steps) mma_commit(smem_u32(&sh.kv_empty[0]));
-      }
-      const int first_open = open_keys / kTile;
-      for (int j = 0; ok && j < steps; ++j) {
-        const int tv = 2 * j + 1, tk = 2 * j + 2;
-        bool v_ready = false, k_ready = false;
-        for (int i = 0; ok && i < 2; ++i) {
-          const int mine = i ? steps1 : steps0;
-          if (j >= mine) continue;
-          if (!v_ready) {
-            ok = full(tv);
-            if (ok && j >= first_open)
-              ok = mbar_wait(smem_u32(&sh.v_clean[tv % C::kStages]), ((j - first_open) / C::kVPeriod) & 1, abort);
-            v_ready = true;
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t at = ((k >> 2) * C::kHalfBytes + (k & 3) * 32) >> 4;
+            mma_ss(tmem + i * kTile, a + at, b + at, qk_idesc, k > 0);
           }
-          if (ok) ok = mbar_wait(smem_u32(&sh.p_full[i]), j & 1, abort);
-          if (!ok) break;
-          tcgen05_after_sync();
-#pragma unroll
-          for (int k = 0; k < kTile / 16; ++k)
-            mma_ts(tmem + 2 * kTile + i * kTile, tmem + i * kTile + k * 8,
-                   smem_desc(v_major, ring + (tv % C::kStages) * C::kTileBytes + k * 2048), pv_idesc, j > 0 || k > 0);
-          if (j + 1 == mine) {
-            mma_commit(smem_u32(&sh.o_full[i]));
-          } else {
-            if (!k_ready) ok = full(tk);
-            k_ready = true;
-            if (ok) qk(i, tk % C::kStages);
-          }
-        }
+          mma_commit(smem_u32(&sh.s_full[i]));
+        };
+        const auto full = [&](int t) {
+          return mbar_wait(smem_u32(&sh.kv_full[t % C::kStages]), (t / C::kStages) & 1, abort);
+        };
+        bool ok = mbar_wait(smem_u32(&sh.q_full), 0, abort) && full(0);
         if (ok) {
-          // (no arrival that nobody waits for: it could come after the CTA is gone)
-          if (tv + C::kStages < 2 * steps) mma_commit(smem_u32(&sh.kv_empty[tv % C::kStages]));
-          if (tk + C::kStages < 2 * steps) mma_commit(smem_u32(&sh.kv_empty[tk % C::kStages]));
+          tcgen05_after_sync();
+          if (steps0 > 0) qk(0, 0);
+          if (steps1 > 0) qk(1, 0);
+          if (C::kStages < 2 * steps) mma_commit(smem_u32(&sh.kv_empty[0]));
         }
-      }
-    }
-  } else if (warp == 10) {
-    // ------------------------------------------------------------ masked V
-    bool fix = false;
-    for (int j = open_keys / kTile; j < steps; ++j) {
-      const int t = 2 * j + 1;
-      // the loads' word that the stage has come to tile t, whose parity then is unmistakable
-      if (!warp_wait(&sh.v_turn[t % C::kStages], ((j - open_keys / kTile) / C::kVPeriod) & 1, abort)) break;
-      if (!warp_wait(&sh.kv_full[t % C::kStages], (t / C::kStages) & 1, abort)) break;
-      const int first = max(open_keys - j * kTile, 0);      // first key that some row may not see
-      const int behind = clamp_to(w.keys - j * kTile, 0, kTile);  // first key behind the sequence
-      for (int h = 0; h < C::kHalves; ++h) {
-        const uint32_t base = ring + (t % C::kStages) * C::kTileBytes + h * C::kHalfBytes;
-        for (int x = first * 8 + lane; x < kTile * 8; x += 32) {
-          const uint32_t at = base + x * 16;
-          uint32_t v[4] = {0, 0, 0, 0};
-          bool write = x >= behind * 8;
-          if (!write) {
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                         : "r"(at));
+        const int first_open = open_keys / kTile;
+        for (int j = 0; ok && j < steps; ++j) {
+          const int tv = 2 * j + 1, tk = 2 * j + 2;
+          bool v_ready = false, k_ready = false;
+          for (int i = 0; ok && i < 2; ++i) {
+            const int mine = i ? steps1 : steps0;
+            if (j >= mine) continue;
+            if (!v_ready) {
+              ok = full(tv);
+              if (ok && j >= first_open)
+                ok = mbar_wait(smem_u32(&sh.v_clean[tv % C::kStages]), ((j - first_open) / C::kVPeriod) & 1, abort);
+              v_ready = true;
+            }
+            uint64_t v = smem_desc(v_major, ring + (tv % C::kStages) * C::kTileBytes);
+            keep_here(v);
+            const auto pv = [&](int k) {
+              mma_ts(tmem + 2 * kTile + i * kTile, tmem + i * kTile + k * 8, v + k * (2048 >> 4), pv_idesc, j > 0 || k > 0);
+            };
+            if (ok) ok = mbar_wait(smem_u32(&sh.p_part[i]), j & 1, abort);
+            if (!ok) break;
+            tcgen05_after_sync();
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              // exponent all ones: infinite or not a number
-              if ((v[e] & 0x7F80u) == 0x7F80u) v[e] &= 0xFFFF0000u, write = fix = true;
-              if ((v[e] & 0x7F800000u) == 0x7F800000u) v[e] &= 0xFFFFu, write = fix = true;
+            for (int k = 0; k < kFirstPart / 16; ++k) pv(k);
+            ok = mbar_wait(smem_u32(&sh.p_full[i]), j & 1, abort);
+            if (!ok) break;
+            tcgen05_after_sync();
+#pragma unroll
+            for (int k = kFirstPart / 16; k < kTile / 16; ++k) pv(k);
+            if (j + 1 == mine) {
+              mma_commit(smem_u32(&sh.o_full[i]));
+            } else {
+              if (!k_ready) ok = full(tk);
+              k_ready = true;
+              if (ok) qk(i, tk % C::kStages);
             }
           }
-          if (write)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-                         "r"(v[3])
-                         : "memory");
+          if (ok) {
+            // (no arrival that nobody waits for: it could come after the CTA is gone)
+            if (tv + C::kStages < 2 * steps) mma_commit(smem_u32(&sh.kv_empty[tv % C::kStages]));
+            if (tk + C::kStages < 2 * steps) mma_commit(smem_u32(&sh.kv_empty[tk % C::kStages]));
+          }
         }
       }
-      fence_proxy_async_shared();
-      fix = __any_sync(0xffffffffu, fix);
-      if (lane == 0) mbar_arrive(smem_u32(&sh.v_clean[t % C::kStages]));
-      __syncwarp();
+    } else if (warp == 10) {
+      // ------------------------------------------------------------ masked V
+      bool fix = false;
+      for (int j = open_keys / kTile; j < steps; ++j) {
+        const int t = 2 * j + 1;
+        // the loads' word that the stage has come to tile t, whose parity then is unmistakable
+        if (!warp_wait(&sh.v_turn[t % C::kStages], ((j - open_keys / kTile) / C::kVPeriod) & 1, abort)) break;
+        if (!warp_wait(&sh.kv_full[t % C::kStages], (t / C::kStages) & 1, abort)) break;
+        const int first = max(open_keys - j * kTile, 0);      // first key that some row may not see
+        const int behind = clamp_to(w.keys - j * kTile, 0, kTile);  // first key behind the sequence
+        for (int h = 0; h < C::kHalves; ++h) {
+          const uint32_t base = ring + (t % C::kStages) * C::kTileBytes + h * C::kHalfBytes;
+          for (int x = first * 8 + lane; x < kTile * 8; x += 32) {
+            const uint32_t at = base + x * 16;
+            uint32_t v[4] = {0, 0, 0, 0};
+            bool write = x >= behind * 8;
+            if (!write) {
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                           : "r"(at));
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                // exponent all ones: infinite or not a number
+                if ((v[e] & 0x7F80u) == 0x7F80u) v[e] &= 0xFFFF0000u, write = fix = true;
+                if ((v[e] & 0x7F800000u) == 0x7F800000u) v[e] &= 0xFFFFu, write = fix = true;
+              }
+            }
+            if (write)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                           "r"(v[3])
+                           : "memory");
+          }
+        }
+        fence_proxy_async_shared();
+        fix = __any_sync(0xffffffffu, fix);
+        if (lane == 0) mbar_arrive(smem_u32(&sh.v_clean[t % C::kStages]));
+        __syncwarp();
+      }
+      if (lane == 0) {
+        if (fix) *reinterpret_cast<volatile int*>(&sh.fix) = 1;
+        mbar_arrive(smem_u32(&sh.fix_done));
+      }
     }
-    if (lane == 0) {
-      if (fix) *reinterpret_cast<volatile int*>(&sh.fix) = 1;
-      mbar_arrive(smem_u32(&sh.fix_done));
-    }
-  } else if (warp < 8) {
+  } else {
     // ------------------------------------------------------------ softmax
+    regs_inc<kSoftmaxRegs>();
     const int i = warp >> 2;
     const int mine = i ? steps1 : steps0;
     const int row = tid & (kTile - 1);
@@ -416,15 +435,15 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
 #pragma unroll
         for (int c = 0; c < kTile; ++c) s[c] = c < limit ? s[c] : -INFINITY;
       }
-      float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
+      float m0 = -INFINITY, m1 = m0, m2 = m0, m3 = m0;
 #pragma unroll
-      for (int c = 4; c < kTile; c += 4) {
-        m0 = fmaxf(m0, s[c]);
-        m1 = fmaxf(m1, s[c + 1]);
-        m2 = fmaxf(m2, s[c + 2]);
-        m3 = fmaxf(m3, s[c + 3]);
+      for (int c = 0; c < kTile; c += 8) {
+        m0 = max3(m0, s[c], s[c + 1]);
+        m1 = max3(m1, s[c + 2], s[c + 3]);
+        m2 = max3(m2, s[c + 4], s[c + 5]);
+        m3 = max3(m3, s[c + 6], s[c + 7]);
       }
-      const float high = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+      const float high = fmaxf(max3(m0, m1, m2), m3);
       if (j == 0) {
         top = high;
       } else if (__any_sync(0xffffffffu, live && (high - top) * scale > kRescaleLog2)) {
@@ -463,6 +482,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           w16[e] = pack_bf16x2(a, b);
         }
         tmem_st16(s_at + c / 2, w16);
+        if (c + 32 == kFirstPart) {
+          tmem_wait_st();
+          tcgen05_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sh.p_part[i]));
+        }
       }
       tmem_wait_st();
       tcgen05_before_sync();
@@ -476,7 +501,6 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       ok = warp_wait(&sh.fix_done, 0, abort) && warp_wait(&sh.o_full[i], 0, abort);
       tcgen05_after_sync();
     }
-    const bool fix = *reinterpret_cast<volatile int*>(&sh.fix) != 0;
     const float inv = mine == 0 || total == 0.f ? 0.f : 1.f / total;
     __nv_bfloat16* out = p.out + (static_cast<int64_t>(w.row0 + t) * p.q_heads + w.head * p.group + row % p.group) * D;
     if (ok && valid > 0) {
@@ -490,11 +514,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         uint32_t x[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          float a = inv == 0.f ? 0.f : o[2 * e] * inv, b = inv == 0.f ? 0.f : o[2 * e + 1] * inv;
-          if (fix && live) {
-            a += non_finite_sum(p, w.seq, w.head, w.row0, D, open_keys, sees, c + 2 * e);
-            b += non_finite_sum(p, w.seq, w.head, w.row0, D, open_keys, sees, c + 2 * e + 1);
-          }
+          const float a = inv == 0.f ? 0.f : o[2 * e] * inv, b = inv == 0.f ? 0.f : o[2 * e + 1] * inv;
           x[e] = pack_bf16x2(a, b);
         }
         if (live) {
@@ -504,6 +524,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         }
       }
     }
+    if (ok && live && *reinterpret_cast<volatile int*>(&sh.fix) != 0)
+      add_non_finite(p, w.seq, w.head, w.row0, D, open_keys, sees, out);
     tcgen05_before_sync();
   }
   __syncthreads();

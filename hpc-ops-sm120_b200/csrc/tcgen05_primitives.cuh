@@ -79,6 +79,10 @@ __device__ __forceinline__ uint64_t smem_desc(uint64_t base, uint32_t addr) {
   return base | static_cast<uint64_t>((addr & 0x3FFFFu) >> 4);
 }
 
+// Keeps the compiler from computing what depends on `x` ahead of this place
+// (descriptors of a whole loop would not fit the issuing warp's registers).
+__device__ __forceinline__ void keep_here(uint64_t& x) { asm volatile("" : "+l"(x)); }
+
 // Instruction descriptor: FP32 accumulator, BF16 A and B, A K-major.
 __host__ __device__ constexpr uint32_t mma_idesc(int m, int n, bool b_mn_major) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn_major ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
@@ -126,7 +130,23 @@ __device__ __forceinline__ void tma_load_tile_4d(uint32_t dst, const CUtensorMap
       : "memory");
 }
 
+// ---------------------------------------------------------------- registers
+// Moves a warpgroup's register count (all its warps execute it).
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // ---------------------------------------------------------------- packed FP32
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 __device__ __forceinline__ uint64_t pack2(float lo, float hi) {
   uint64_t v;
   asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
