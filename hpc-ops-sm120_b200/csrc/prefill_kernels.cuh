@@ -152,9 +152,12 @@ __device__ __forceinline__ int tile_steps(const PrefillParams& p, const PrefillW
   return valid > 0 && last > 0 ? (last + kTile - 1) / kTile : 0;
 }
 
-// A wait of a whole warp, with one answer for all lanes.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, abort));
+// A wait that goes on in any case: when it runs out (mbar_wait) the abort flag
+// is set, every later wait ends at once, no more loads are started and nothing
+// is written.
+__device__ __forceinline__ void wait_or_abort(const uint64_t* bar, uint32_t parity, volatile int* abort) {
+  mbar_wait(smem_u32(bar), parity, abort);
+  __syncwarp();
 }
 
 // Adds the non-finite values of V[key][d], key in [lo, hi), that were cleared
@@ -257,7 +260,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         for (int t = 0; t < 2 * steps; ++t) {
           const int stage = t % C::kStages;
           if (t >= C::kStages) {
-            if (!warp_wait(&sh.kv_empty[stage], (t / C::kStages - 1) & 1, abort)) break;
+            wait_or_abort(&sh.kv_empty[stage], (t / C::kStages - 1) & 1, abort);
+            if (__any_sync(0xffffffffu, *abort)) break;
           }
           const int key0 = (t >> 1) * kTile;
           const uint32_t bar = smem_u32(&sh.kv_full[stage]);
@@ -293,73 +297,77 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       }
     } else if (warp == 9) {
       // ------------------------------------------------------------ products
-      if (lane == 0 && steps > 0) {
+      // The whole warp runs the loop, so that the compiler sees uniform values
+      // (descriptors in uniform registers); one lane issues.  With the loop in
+      // one lane's branch an MMA took 65 cycles to issue, and the issue was
+      // what bounded the kernel (567 us for 8192 tokens, 32/8 heads, D 128).
+      if (steps > 0) {
         constexpr uint64_t k_major = smem_desc_base(16, 1024);
         constexpr uint64_t v_major = smem_desc_base(C::kHalfBytes, 1024);
         constexpr uint32_t qk_idesc = mma_idesc(kTile, kTile, false);
         constexpr uint32_t pv_idesc = mma_idesc(kTile, D, true);
         const auto qk = [&](int i, int stage) {
-          uint64_t a = smem_desc(k_major, tiles + i * C::kTileBytes), b = smem_desc(k_major, ring + stage * C::kTileBytes);
-          keep_here(a);
-          keep_here(b);
+          const uint64_t a = smem_desc(k_major, tiles + i * C::kTileBytes);
+          const uint64_t b = smem_desc(k_major, ring + stage * C::kTileBytes);
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t at = ((k >> 2) * C::kHalfBytes + (k & 3) * 32) >> 4;
-            mma_ss(tmem + i * kTile, a + at, b + at, qk_idesc, k > 0);
+            for (int k = 0; k < D / 16; ++k) {
+              const uint32_t at = ((k >> 2) * C::kHalfBytes + (k & 3) * 32) >> 4;
+              mma_ss(tmem + i * kTile, a + at, b + at, qk_idesc, k > 0);
+            }
+            mma_commit(smem_u32(&sh.s_full[i]));
           }
-          mma_commit(smem_u32(&sh.s_full[i]));
+          __syncwarp();
         };
-        const auto full = [&](int t) {
-          return mbar_wait(smem_u32(&sh.kv_full[t % C::kStages]), (t / C::kStages) & 1, abort);
+        const auto pv = [&](int i, int stage, int first, int last, bool accumulate) {
+          const uint64_t v = smem_desc(v_major, ring + stage * C::kTileBytes);
+          if (elect_one()) {
+#pragma unroll
+            for (int k = first; k < last; ++k)
+              mma_ts(tmem + 2 * kTile + i * kTile, tmem + i * kTile + k * 8, v + k * (2048 >> 4), pv_idesc,
+                     accumulate || k > 0);
+          }
+          __syncwarp();
         };
-        bool ok = mbar_wait(smem_u32(&sh.q_full), 0, abort) && full(0);
-        if (ok) {
-          tcgen05_after_sync();
-          if (steps0 > 0) qk(0, 0);
-          if (steps1 > 0) qk(1, 0);
-          if (C::kStages < 2 * steps) mma_commit(smem_u32(&sh.kv_empty[0]));
-        }
+        const auto release = [&](int t) {
+          // (no arrival that nobody waits for: it could come after the CTA is gone)
+          if (t + C::kStages < 2 * steps && elect_one()) mma_commit(smem_u32(&sh.kv_empty[t % C::kStages]));
+          __syncwarp();
+        };
         const int first_open = open_keys / kTile;
-        for (int j = 0; ok && j < steps; ++j) {
-          const int tv = 2 * j + 1, tk = 2 * j + 2;
-          bool v_ready = false, k_ready = false;
-          for (int i = 0; ok && i < 2; ++i) {
+        wait_or_abort(&sh.q_full, 0, abort);
+        wait_or_abort(&sh.kv_full[0], 0, abort);
+        tcgen05_after_sync();
+        if (steps0 > 0) qk(0, 0);
+        if (steps1 > 0) qk(1, 0);
+        release(0);
+        int v_stage = 1, k_stage = 2, v_phase = 0, k_phase = 0;
+        for (int j = 0; j < steps; ++j) {
+          wait_or_abort(&sh.kv_full[v_stage], v_phase, abort);
+          if (j >= first_open) wait_or_abort(&sh.v_clean[v_stage], ((j - first_open) / C::kVPeriod) & 1, abort);
+          if (j + 1 < steps) wait_or_abort(&sh.kv_full[k_stage], k_phase, abort);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
             const int mine = i ? steps1 : steps0;
             if (j >= mine) continue;
-            if (!v_ready) {
-              ok = full(tv);
-              if (ok && j >= first_open)
-                ok = mbar_wait(smem_u32(&sh.v_clean[tv % C::kStages]), ((j - first_open) / C::kVPeriod) & 1, abort);
-              v_ready = true;
-            }
-            uint64_t v = smem_desc(v_major, ring + (tv % C::kStages) * C::kTileBytes);
-            keep_here(v);
-            const auto pv = [&](int k) {
-              mma_ts(tmem + 2 * kTile + i * kTile, tmem + i * kTile + k * 8, v + k * (2048 >> 4), pv_idesc, j > 0 || k > 0);
-            };
-            if (ok) ok = mbar_wait(smem_u32(&sh.p_part[i]), j & 1, abort);
-            if (!ok) break;
+            wait_or_abort(&sh.p_part[i], j & 1, abort);
             tcgen05_after_sync();
-#pragma unroll
-            for (int k = 0; k < kFirstPart / 16; ++k) pv(k);
-            ok = mbar_wait(smem_u32(&sh.p_full[i]), j & 1, abort);
-            if (!ok) break;
+            pv(i, v_stage, 0, kFirstPart / 16, j > 0);
+            wait_or_abort(&sh.p_full[i], j & 1, abort);
             tcgen05_after_sync();
-#pragma unroll
-            for (int k = kFirstPart / 16; k < kTile / 16; ++k) pv(k);
-            if (j + 1 == mine) {
+            pv(i, v_stage, kFirstPart / 16, kTile / 16, true);
+            if (j + 1 < mine) {
+              qk(i, k_stage);
+            } else if (elect_one()) {
               mma_commit(smem_u32(&sh.o_full[i]));
-            } else {
-              if (!k_ready) ok = full(tk);
-              k_ready = true;
-              if (ok) qk(i, tk % C::kStages);
             }
+            __syncwarp();
           }
-          if (ok) {
-            // (no arrival that nobody waits for: it could come after the CTA is gone)
-            if (tv + C::kStages < 2 * steps) mma_commit(smem_u32(&sh.kv_empty[tv % C::kStages]));
-            if (tk + C::kStages < 2 * steps) mma_commit(smem_u32(&sh.kv_empty[tk % C::kStages]));
-          }
+          release(2 * j + 1);
+          release(2 * j + 2);
+          v_stage += 2, k_stage += 2;
+          if (v_stage >= C::kStages) v_stage -= C::kStages, v_phase ^= 1;
+          if (k_stage >= C::kStages) k_stage -= C::kStages, k_phase ^= 1;
         }
       }
     } else if (warp == 10) {
@@ -368,8 +376,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       for (int j = open_keys / kTile; j < steps; ++j) {
         const int t = 2 * j + 1;
         // the loads' word that the stage has come to tile t, whose parity then is unmistakable
-        if (!warp_wait(&sh.v_turn[t % C::kStages], ((j - open_keys / kTile) / C::kVPeriod) & 1, abort)) break;
-        if (!warp_wait(&sh.kv_full[t % C::kStages], (t / C::kStages) & 1, abort)) break;
+        wait_or_abort(&sh.v_turn[t % C::kStages], ((j - open_keys / kTile) / C::kVPeriod) & 1, abort);
+        wait_or_abort(&sh.kv_full[t % C::kStages], (t / C::kStages) & 1, abort);
         const int first = max(open_keys - j * kTile, 0);      // first key that some row may not see
         const int behind = clamp_to(w.keys - j * kTile, 0, kTile);  // first key behind the sequence
         for (int h = 0; h < C::kHalves; ++h) {
@@ -421,10 +429,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     const uint32_t s_at = tmem + i * kTile + lanes, o_at = tmem + 2 * kTile + i * kTile + lanes;
     const float scale = p.scale_log2;
     float top = -INFINITY, total = 0.f;
-    bool ok = true;
     for (int j = 0; j < mine; ++j) {
-      ok = warp_wait(&sh.s_full[i], j & 1, abort);
-      if (!ok) break;
+      wait_or_abort(&sh.s_full[i], j & 1, abort);
       tcgen05_after_sync();
       float s[kTile];
 #pragma unroll
@@ -497,10 +503,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       unpack2(add2(sum0, sum1), a, b);
       total += a + b;
     }
-    if (mine > 0 && ok) {
-      ok = warp_wait(&sh.fix_done, 0, abort) && warp_wait(&sh.o_full[i], 0, abort);
+    if (mine > 0) {
+      wait_or_abort(&sh.fix_done, 0, abort);
+      wait_or_abort(&sh.o_full[i], 0, abort);
       tcgen05_after_sync();
     }
+    const bool ok = __all_sync(0xffffffffu, *abort == 0);
     const float inv = mine == 0 || total == 0.f ? 0.f : 1.f / total;
     __nv_bfloat16* out = p.out + (static_cast<int64_t>(w.row0 + t) * p.q_heads + w.head * p.group + row % p.group) * D;
     if (ok && valid > 0) {
@@ -530,6 +538,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   }
   __syncthreads();
   griddep_launch_dependents();
+  if (*abort != 0) __nanosleep(1000000);  // after a wait that ran out: what was still in flight
   if (warp == 9) {
     tcgen05_after_sync();
     tmem_dealloc(tmem, 512);

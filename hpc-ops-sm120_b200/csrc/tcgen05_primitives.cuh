@@ -79,9 +79,14 @@ __device__ __forceinline__ uint64_t smem_desc(uint64_t base, uint32_t addr) {
   return base | static_cast<uint64_t>((addr & 0x3FFFFu) >> 4);
 }
 
-// Keeps the compiler from computing what depends on `x` ahead of this place
-// (descriptors of a whole loop would not fit the issuing warp's registers).
-__device__ __forceinline__ void keep_here(uint64_t& x) { asm volatile("" : "+l"(x)); }
+// One lane of a converged warp, always the same one.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
 
 // Instruction descriptor: FP32 accumulator, BF16 A and B, A K-major.
 __host__ __device__ constexpr uint32_t mma_idesc(int m, int n, bool b_mn_major) {
