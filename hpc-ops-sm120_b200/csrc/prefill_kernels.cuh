@@ -16,7 +16,7 @@
 //   warps 0-3, 4-7   softmax of tile 0, 1: one thread per row
 //   warp 8           TMA loads: Q once, then K_0 V_0 K_1 V_1 ... into a ring
 //   warp 9           issues the tensor-core products (one thread)
-//   warp 10          clears masked V rows of border tiles (below)
+//   warps 10, 11     clear masked V rows of border tiles (below)
 // S_i = Q_i K_j^T (FP32) and O_i live in tensor memory; the softmax thread
 // reads its row of S_i, writes the weights P_i (BF16) over it, and the product
 // O_i += P_i V_j takes P_i from tensor memory.  While one tile's softmax runs
@@ -160,6 +160,24 @@ __device__ __forceinline__ void wait_or_abort(const uint64_t* bar, uint32_t pari
   __syncwarp();
 }
 
+// Two bf16 values: a bit of either half is set if that value's exponent is all
+// ones (infinite or not a number).
+__device__ __forceinline__ uint32_t non_finite_bits(uint32_t x) { return ((x & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }
+__device__ __forceinline__ uint32_t finite_or_zero(uint32_t x) {
+  const uint32_t bad = non_finite_bits(x);
+  return x & ~((bad & 0x8000u ? 0xFFFFu : 0u) | (bad & 0x80000000u ? 0xFFFF0000u : 0u));
+}
+
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, const uint4& v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+               : "memory");
+}
+
 // Adds the non-finite values of V[key][d], key in [lo, hi), that were cleared
 // for the tile to the row `out` that sees them.
 __device__ __noinline__ void add_non_finite(const PrefillParams& p, int seq, int head, int row0, int dim, int lo,
@@ -201,7 +219,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       mbar_init(smem_u32(&sh.kv_full[s]), 1);
       mbar_init(smem_u32(&sh.kv_empty[s]), 1);
       mbar_init(smem_u32(&sh.v_turn[s]), 1);
-      mbar_init(smem_u32(&sh.v_clean[s]), 1);
+      mbar_init(smem_u32(&sh.v_clean[s]), 2);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&sh.s_full[i]), 1);
@@ -209,7 +227,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       mbar_init(smem_u32(&sh.p_full[i]), 4);
       mbar_init(smem_u32(&sh.o_full[i]), 1);
     }
-    mbar_init(smem_u32(&sh.fix_done), 1);
+    mbar_init(smem_u32(&sh.fix_done), 2);
     sh.abort = 0;
     sh.fix = 0;
     fence_barrier_init();
@@ -370,48 +388,55 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           if (k_stage >= C::kStages) k_stage -= C::kStages, k_phase ^= 1;
         }
       }
-    } else if (warp == 10) {
+    } else {
       // ------------------------------------------------------------ masked V
+      // Warps 10 and 11 take every other 128 vectors of 16 bytes.
       bool fix = false;
       for (int j = open_keys / kTile; j < steps; ++j) {
         const int t = 2 * j + 1;
         // the loads' word that the stage has come to tile t, whose parity then is unmistakable
         wait_or_abort(&sh.v_turn[t % C::kStages], ((j - open_keys / kTile) / C::kVPeriod) & 1, abort);
         wait_or_abort(&sh.kv_full[t % C::kStages], (t / C::kStages) & 1, abort);
-        const int first = max(open_keys - j * kTile, 0);      // first key that some row may not see
-        const int behind = clamp_to(w.keys - j * kTile, 0, kTile);  // first key behind the sequence
+        const int first = 8 * max(open_keys - j * kTile, 0);            // first vector that some row may not see
+        const int behind = 8 * clamp_to(w.keys - j * kTile, 0, kTile);  // first vector behind the sequence
         for (int h = 0; h < C::kHalves; ++h) {
           const uint32_t base = ring + (t % C::kStages) * C::kTileBytes + h * C::kHalfBytes;
-          for (int x = first * 8 + lane; x < kTile * 8; x += 32) {
-            const uint32_t at = base + x * 16;
-            uint32_t v[4] = {0, 0, 0, 0};
-            bool write = x >= behind * 8;
-            if (!write) {
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                           : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                           : "r"(at));
+          for (int x0 = (warp - 10) * 128 + lane; x0 < kTile * 8; x0 += 256) {
+            uint4 v[4];
+            uint32_t bad = 0;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                // exponent all ones: infinite or not a number
-                if ((v[e] & 0x7F80u) == 0x7F80u) v[e] &= 0xFFFF0000u, write = fix = true;
-                if ((v[e] & 0x7F800000u) == 0x7F800000u) v[e] &= 0xFFFFu, write = fix = true;
+            for (int u = 0; u < 4; ++u) {
+              const int x = x0 + 32 * u;
+              v[u] = make_uint4(0, 0, 0, 0);
+              if (x >= first && x < behind) v[u] = ld_shared_v4(base + x * 16);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              bad |= non_finite_bits(v[u].x) | non_finite_bits(v[u].y) | non_finite_bits(v[u].z) | non_finite_bits(v[u].w);
+            if (bad != 0) {
+              fix = true;
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                const int x = x0 + 32 * u;
+                if (x >= first && x < behind)
+                  st_shared_v4(base + x * 16, make_uint4(finite_or_zero(v[u].x), finite_or_zero(v[u].y),
+                                                         finite_or_zero(v[u].z), finite_or_zero(v[u].w)));
               }
             }
-            if (write)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-                           "r"(v[3])
-                           : "memory");
+            if (x0 + 96 >= behind) {
+#pragma unroll
+              for (int u = 0; u < 4; ++u)
+                if (x0 + 32 * u >= behind) st_shared_v4(base + (x0 + 32 * u) * 16, make_uint4(0, 0, 0, 0));
+            }
           }
         }
         fence_proxy_async_shared();
-        fix = __any_sync(0xffffffffu, fix);
-        if (lane == 0) mbar_arrive(smem_u32(&sh.v_clean[t % C::kStages]));
         __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.v_clean[t % C::kStages]));
       }
-      if (lane == 0) {
-        if (fix) *reinterpret_cast<volatile int*>(&sh.fix) = 1;
-        mbar_arrive(smem_u32(&sh.fix_done));
-      }
+      if (fix) *reinterpret_cast<volatile int*>(&sh.fix) = 1;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.fix_done));
     }
   } else {
     // ------------------------------------------------------------ softmax
