@@ -28,6 +28,8 @@ using adb_host::DeviceGuard;
 using adb_host::fail;
 using adb_host::is_aligned;
 
+constexpr int64_t kL2Bytes = 126 << 20;
+
 int check_heads(int64_t total, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim) {
   if (total <= 0 || batch <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0)
     return fail(ADB_ERR_INVALID_ARGUMENT,
@@ -135,6 +137,11 @@ int launch(adb::PrefillParams& p, const void* q, int64_t q_token, int64_t q_head
   // every sequence with a token may end in a partly filled pair of tiles
   const int64_t per = 2 * p.tile_tokens;
   const int64_t pairs = p.total / per + std::min(p.batch, p.total);
+  // KV heads worked on at a time: as many as keep the longest possible
+  // sequence's K and V within half of L2
+  const int64_t keys = p.paged ? int64_t(p.max_blocks) << p.page_shift : p.total;
+  p.head_group = static_cast<int>(
+      std::max<int64_t>(1, std::min<int64_t>(p.kv_heads, kL2Bytes / 2 / std::max<int64_t>(1, keys * dim * 4))));
   if (pairs * p.kv_heads > INT32_MAX) return fail(ADB_ERR_INVALID_ARGUMENT, "too many tiles for one call");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(pairs * p.kv_heads));

@@ -12,10 +12,17 @@
 // fill tiles; any G up to 64 works.  A CTA owns two such tiles of one
 // (sequence, KV head) and streams the K/V tiles (128 keys) that they see.
 //
+// Work.  A unit is a pair of tiles of one (sequence, KV head), or a part of
+// its K/V tiles (below).  The grid has a CTA for every unit there can be; a
+// running CTA takes over units whose CTA has not started (cluster launch
+// control), so that one CTA's loads and first products overlap the end of its
+// unit before.  Units that see the most keys come first.
+//
 // Pipeline of a CTA (384 threads):
 //   warps 0-3, 4-7   softmax of tile 0, 1: one thread per row
-//   warp 8           TMA loads: Q once, then K_0 V_0 K_1 V_1 ... into a ring
-//   warp 9           issues the tensor-core products (one thread)
+//   warp 8           finds the units; TMA loads: Q, then K_0 V_0 K_1 V_1 ...
+//                    into a ring that runs on over the units
+//   warp 9           issues the tensor-core products
 //   warps 10, 11     clear masked V rows of border tiles (below)
 // S_i = Q_i K_j^T (FP32) and O_i live in tensor memory; the softmax thread
 // reads its row of S_i, writes the weights P_i (BF16) over it, and the product
@@ -54,6 +61,7 @@ struct PrefillParams {
   int64_t table_stride;
   int total, batch, q_heads, kv_heads, group;
   int tile_tokens;         // tokens of a Q tile: 128 / group
+  int head_group;          // KV heads that are worked on at a time
   int paged;               // 0 packed K/V, 1 HND pages, 2 NHD pages
   int max_blocks, num_blocks, page_shift;
   float scale_log2;        // log2(e) / sqrt(D)
@@ -65,32 +73,39 @@ struct PrefillCfg {
   static constexpr int kHalfBytes = kTile * 128;             // one column block of a tile
   static constexpr int kTileBytes = kHalves * kHalfBytes;
   static constexpr int kStages = D == 128 ? 5 : 8;           // K and V tiles in flight
-  static constexpr int kVPeriod = kStages % 2 ? kStages : kStages / 2;  // V tiles until a stage holds V again
   static constexpr int kSmemBytes = (2 + kStages) * kTileBytes + 1024;
 };
 
 // What a CTA works on.
 struct PrefillWork {
-  int seq, head;     // sequence, KV head (seq < 0: nothing)
+  int seq, head;     // sequence, KV head; seq -1: only padding, -2: no more work
+  int index;         // of the unit (its share of the padding)
   int row0;          // first row of the sequence in q / out
   int token0;        // first token of tile 0, within the sequence's new ones
-  int tokens;        // new tokens of the sequence
-  int before;        // keys before token 0 (may be negative)
+  int before;        // keys before the sequence's token 0 (may be negative)
   int keys;          // keys of the sequence
+  int valid[2];      // tokens of the tiles
+  int first;         // K/V tiles first .. first + steps[i] - 1 are tile i's
+  int steps[2];
+  int open_keys;     // keys from here on are hidden from some row of the tiles
+  int pad_head, pad_tail;  // rows before the first / from the end of the last sequence
 };
 
 template <int D>
 struct PrefillShared {
-  alignas(8) uint64_t q_full;
+  alignas(16) uint4 next;  // cluster launch control's answer
+  uint64_t next_full;
+  uint64_t work_full[2], work_empty[2];
+  uint64_t q_full, q_empty;
   uint64_t kv_full[PrefillCfg<D>::kStages], kv_empty[PrefillCfg<D>::kStages];
   uint64_t s_full[2], p_part[2], p_full[2], o_full[2];
   uint64_t v_turn[PrefillCfg<D>::kStages];   // a border tile of V is on its way
   uint64_t v_clean[PrefillCfg<D>::kStages];  // and cleared
-  uint64_t fix_done;
+  uint64_t fix_done[2];
   uint32_t tmem;
   int abort;
-  int fix;           // a non-finite value of V was cleared
-  PrefillWork work;
+  int fix[2];        // number of the unit of which a non-finite value of V was cleared
+  PrefillWork work[2];
 };
 
 __device__ __forceinline__ int clamp_to(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }
@@ -101,55 +116,161 @@ __device__ __forceinline__ void sequence_rows(const PrefillParams& p, int b, int
   count = clamp_to(p.cu[b + 1], first, p.total) - first;
 }
 
-// The item-th pair of tiles over all sequences (one warp; the result is the
-// same in all lanes).
-__device__ __forceinline__ void find_work(const PrefillParams& p, int index, PrefillWork& w) {
+// The units of all sequences, held by one warp: lane l has sequences l, l + 32,
+// ...  Pair i of a sequence is on level base + i + 1, the keys that it sees in
+// units of a pair's tokens, and higher levels come first: with counts F(l) of
+// the pairs above a level, a pair is found by bisection and no list is needed.
+// Larger batches, whose many sequences fill the GPU in any order, are walked
+// in their order.
+constexpr int kPlanRows = 8;
+struct PrefillPlan {
+  int pairs[kPlanRows], base[kPlanRows];
+  int units;                       // pairs of all sequences
+  int top;                         // highest level
+  int scan_base, scan_before;      // where the walk stands
+};
+
+__device__ __forceinline__ bool plan_is_sorted(const PrefillParams& p) { return p.batch <= 32 * kPlanRows; }
+
+__device__ __forceinline__ int sequence_keys(const PrefillParams& p, int b, int count) {
+  return p.paged ? clamp_to(p.lens[b], 0, p.max_blocks << p.page_shift) : count;
+}
+
+__device__ __forceinline__ void make_plan(const PrefillParams& p, PrefillPlan& plan) {
   const int lane = threadIdx.x & 31;
-  const int item = index / p.kv_heads;
   const int per = 2 * p.tile_tokens;
-  w.head = index - item * p.kv_heads;
-  w.seq = -1;
-  int before = 0;
-  for (int base = 0; base < p.batch; base += 32) {
-    int first = 0, count = 0;
-    if (base + lane < p.batch) sequence_rows(p, base + lane, first, count);
-    const int mine = (count + per - 1) / per;
-    int inc = mine;
+  plan.scan_base = plan.scan_before = 0;
+  int units = 0, top = 0;
+  if (plan_is_sorted(p)) {
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, inc, d);
-      if (lane >= d) inc += o;
+    for (int r = 0; r < kPlanRows; ++r) {
+      plan.pairs[r] = plan.base[r] = 0;
+      const int b = 32 * r + lane;
+      if (b < p.batch) {
+        int first, count;
+        sequence_rows(p, b, first, count);
+        plan.pairs[r] = (count + per - 1) / per;
+        plan.base[r] = max(sequence_keys(p, b, count) - count, 0) / per;
+        units += plan.pairs[r];
+        top = max(top, plan.base[r] + plan.pairs[r]);
+      }
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, item < before + inc);
+  } else {
+    for (int b = lane; b < p.batch; b += 32) {
+      int first, count;
+      sequence_rows(p, b, first, count);
+      units += (count + per - 1) / per;
+    }
+  }
+  plan.units = __reduce_add_sync(0xffffffffu, units);
+  plan.top = __reduce_max_sync(0xffffffffu, top);
+}
+
+// Inclusive prefix of v over the warp.
+__device__ __forceinline__ int warp_prefix(int v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, v, d);
+    if (lane >= d) v += o;
+  }
+  return v;
+}
+
+// Sequence and pair of the r-th unit of the plan (r < units).
+__device__ __forceinline__ void find_pair(const PrefillParams& p, PrefillPlan& plan, int r, int& seq, int& pair) {
+  const int lane = threadIdx.x & 31;
+  if (plan_is_sorted(p)) {
+    // lowest level with at most r pairs above it
+    int lo = 0, hi = plan.top, above = 0;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      int n = 0;
+#pragma unroll
+      for (int s = 0; s < kPlanRows; ++s) n += clamp_to(plan.base[s] + plan.pairs[s] - mid, 0, plan.pairs[s]);
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (n <= r)
+        hi = mid, above = n;
+      else
+        lo = mid;
+    }
+    int k = r - above;
+    seq = pair = 0;
+    bool found = false;
+#pragma unroll
+    for (int s = 0; s < kPlanRows; ++s) {
+      const bool here = plan.base[s] < hi && hi <= plan.base[s] + plan.pairs[s];
+      const unsigned all = __ballot_sync(0xffffffffu, here);
+      const int n = __popc(all);
+      if (!found && k < n) {
+        found = true;
+        const unsigned mine = __ballot_sync(0xffffffffu, here && __popc(all & ((1u << lane) - 1)) == k);
+        const int l = __ffs(mine) - 1;
+        seq = 32 * s + l;
+        pair = hi - __shfl_sync(0xffffffffu, plan.base[s], l) - 1;
+      }
+      k -= n;
+    }
+    return;
+  }
+  const int per = 2 * p.tile_tokens;
+  if (r < plan.scan_before) plan.scan_base = plan.scan_before = 0;
+  for (;;) {
+    const int b = plan.scan_base + lane;
+    int first = 0, count = 0;
+    if (b < p.batch) sequence_rows(p, b, first, count);
+    const int mine = (count + per - 1) / per;
+    const int inc = warp_prefix(mine);
+    const unsigned hit = __ballot_sync(0xffffffffu, r < plan.scan_before + inc);
     if (hit) {
       const int l = __ffs(hit) - 1;
-      w.seq = base + l;
-      w.row0 = __shfl_sync(0xffffffffu, first, l);
-      w.tokens = __shfl_sync(0xffffffffu, count, l);
-      const int items = __shfl_sync(0xffffffffu, mine, l);
-      const int at = item - before - (__shfl_sync(0xffffffffu, inc, l) - items);
-      w.token0 = (items - 1 - at) * per;  // the pair that sees the most keys first
-      break;
+      seq = plan.scan_base + l;
+      const int pairs = __shfl_sync(0xffffffffu, mine, l);
+      const int at = r - plan.scan_before - (__shfl_sync(0xffffffffu, inc, l) - pairs);
+      pair = pairs - 1 - at;  // the one that sees the most keys first
+      return;
     }
-    before += __shfl_sync(0xffffffffu, inc, 31);
+    plan.scan_before += __shfl_sync(0xffffffffu, inc, 31);
+    plan.scan_base += 32;
+    if (plan.scan_base >= p.batch) {  // not reached while r < units
+      seq = -1;
+      pair = 0;
+      return;
+    }
   }
-  if (w.seq < 0) return;
-  w.keys = w.tokens;
-  if (p.paged) w.keys = clamp_to(p.lens[w.seq], 0, p.max_blocks << p.page_shift);
-  w.before = w.keys - w.tokens;
 }
 
-// Keys that token t of the work's sequence sees (0 or less: none).
+// Keys that token t of the unit's sequence sees (0 or less: none).
 __device__ __forceinline__ int keys_of(const PrefillWork& w, int t) { return w.before + t + 1; }
 
-// Valid tokens of tile i and the K/V tiles that it needs.
-__device__ __forceinline__ int tile_valid(const PrefillParams& p, const PrefillWork& w, int i) {
-  return clamp_to(w.tokens - w.token0 - i * p.tile_tokens, 0, p.tile_tokens);
-}
-__device__ __forceinline__ int tile_steps(const PrefillParams& p, const PrefillWork& w, int i) {
-  const int valid = tile_valid(p, w, i);
-  const int last = keys_of(w, w.token0 + i * p.tile_tokens + valid - 1);
-  return valid > 0 && last > 0 ? (last + kTile - 1) / kTile : 0;
+// The index-th unit.  Heads are the fastest index within a group of heads whose
+// K and V stay in L2 together.
+__device__ __forceinline__ void find_work(const PrefillParams& p, PrefillPlan& plan, int index, PrefillWork& w) {
+  w.index = index;
+  w.seq = -1;
+  w.first = w.steps[0] = w.steps[1] = w.valid[0] = w.valid[1] = 0;
+  w.head = w.row0 = w.token0 = w.before = w.keys = w.open_keys = 0;
+  if (index >= plan.units * p.kv_heads) return;
+  const int heads0 = index / (plan.units * p.head_group) * p.head_group;
+  const int heads = min(p.head_group, p.kv_heads - heads0);
+  const int at = index - heads0 * plan.units;
+  w.head = heads0 + at % heads;
+  int pair;
+  find_pair(p, plan, at / heads, w.seq, pair);
+  if (w.seq < 0) return;
+  int count;
+  sequence_rows(p, w.seq, w.row0, count);
+  w.keys = sequence_keys(p, w.seq, count);
+  w.before = w.keys - count;
+  w.token0 = pair * 2 * p.tile_tokens;
+  w.open_keys = max(keys_of(w, w.token0), 0);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int t = w.token0 + i * p.tile_tokens;
+    w.valid[i] = clamp_to(count - t, 0, p.tile_tokens);
+    const int last = keys_of(w, t + w.valid[i] - 1);
+    w.steps[i] = w.valid[i] > 0 && last > 0 ? (last + kTile - 1) / kTile : 0;
+  }
 }
 
 // A wait that goes on in any case: when it runs out (mbar_wait) the abort flag
@@ -205,6 +326,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                    const __grid_constant__ CUtensorMap v_map, const __grid_constant__ PrefillParams p) {
   using C = PrefillCfg<D>;
+  constexpr int S = C::kStages;
   extern __shared__ uint8_t raw[];
   __shared__ PrefillShared<D> sh;
   const int tid = threadIdx.x, lane = tid & 31;
@@ -214,83 +336,114 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   volatile int* abort = &sh.abort;
 
   if (tid == 0) {
-    mbar_init(smem_u32(&sh.q_full), 1);
-    for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(smem_u32(&sh.kv_full[s]), 1);
-      mbar_init(smem_u32(&sh.kv_empty[s]), 1);
-      mbar_init(smem_u32(&sh.v_turn[s]), 1);
-      mbar_init(smem_u32(&sh.v_clean[s]), 2);
+    const auto init = [](uint64_t& bar, int count) { mbar_init(smem_u32(&bar), count); };
+    init(sh.next_full, 1);
+    init(sh.q_full, 1);
+    init(sh.q_empty, 1);
+    for (int s = 0; s < S; ++s) {
+      init(sh.kv_full[s], 1);
+      init(sh.kv_empty[s], 1);
+      init(sh.v_turn[s], 1);
+      init(sh.v_clean[s], 2);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_u32(&sh.s_full[i]), 1);
-      mbar_init(smem_u32(&sh.p_part[i]), 4);
-      mbar_init(smem_u32(&sh.p_full[i]), 4);
-      mbar_init(smem_u32(&sh.o_full[i]), 1);
+      init(sh.work_full[i], 1);
+      init(sh.work_empty[i], 11);
+      init(sh.s_full[i], 1);
+      init(sh.p_part[i], 4);
+      init(sh.p_full[i], 4);
+      init(sh.o_full[i], 1);
+      init(sh.fix_done[i], 2);
     }
-    mbar_init(smem_u32(&sh.fix_done), 2);
     sh.abort = 0;
-    sh.fix = 0;
+    sh.fix[0] = sh.fix[1] = 0;
     fence_barrier_init();
   }
   if (warp == 9) tmem_alloc(smem_u32(&sh.tmem), 512);
-  griddep_wait();
-  if (warp == 8) {
-    PrefillWork w;
-    find_work(p, blockIdx.x, w);
-    if (lane == 0) sh.work = w;
-  }
-  // padding: rows before the first and behind the last sequence
-  {
-    const int from = clamp_to(p.cu[p.batch], 0, p.total), head = clamp_to(p.cu[0], 0, p.total);
-    const int64_t vecs = static_cast<int64_t>(p.q_heads) * (D / 8);
-    uint4* o = reinterpret_cast<uint4*>(p.out);
-    const int64_t step = static_cast<int64_t>(gridDim.x) * kPrefillThreads;
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * kPrefillThreads + tid;
-    for (int64_t i = from * vecs + at; i < p.total * vecs; i += step) o[i] = make_uint4(0, 0, 0, 0);
-    for (int64_t i = at; i < head * vecs; i += step) o[i] = make_uint4(0, 0, 0, 0);
+  if (warp == 8 && lane == 0) {
+    prefetch_tensormap(&q_map);
+    prefetch_tensormap(&k_map);
+    prefetch_tensormap(&v_map);
   }
   tcgen05_before_sync();
   __syncthreads();
   tcgen05_after_sync();
-  const PrefillWork w = sh.work;
   const uint32_t tmem = sh.tmem;
-  const int steps0 = w.seq < 0 ? 0 : tile_steps(p, w, 0), steps1 = w.seq < 0 ? 0 : tile_steps(p, w, 1);
-  const int steps = max(steps0, steps1);
-  // keys from here on are hidden from some row of the tiles
-  const int open_keys = w.seq < 0 ? 0 : max(keys_of(w, w.token0), 0);
+  griddep_wait();
+
+  // Whether there is a unit of turn n (0, 1, ...), in sh.work[n & 1] until
+  // work_done(n); for every warp but the loading one.
+  const auto next_work = [&](int n) {
+    wait_or_abort(&sh.work_full[n & 1], (n >> 1) & 1, abort);
+    return !__any_sync(0xffffffffu, *abort != 0 || sh.work[n & 1].seq == -2);
+  };
+  const auto work_done = [&](int n) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&sh.work_empty[n & 1]));
+  };
 
   if (warp >= 8) {
     regs_dec<kOtherRegs>();
     if (warp == 8) {
       // ------------------------------------------------------------ loads
-      if (steps > 0) {
-        const int boxes = p.paged ? max(1, kTile >> p.page_shift) : 1;
-        const int box_rows = kTile / boxes;
-        if (lane == 0) {
-          const uint32_t bar = smem_u32(&sh.q_full);
-          const int n = steps1 > 0 ? 2 : 1;
-          mbar_arrive_expect_tx(bar, n * C::kHalves * p.tile_tokens * p.group * 128);
-          for (int i = 0; i < n; ++i)
-            for (int h = 0; h < C::kHalves; ++h)
-              tma_load_tile_3d(tiles + i * C::kTileBytes + h * C::kHalfBytes, &q_map, h * 64, w.head * p.group,
-                                w.row0 + w.token0 + i * p.tile_tokens, bar);
+      PrefillPlan plan;
+      make_plan(p, plan);
+      const int pad_tail = clamp_to(p.cu[p.batch], 0, p.total), pad_head = clamp_to(p.cu[0], 0, p.total);
+      const bool pads = pad_tail < p.total || pad_head > 0;
+      const int boxes = p.paged ? max(1, kTile >> p.page_shift) : 1;
+      const int box_rows = kTile / boxes;
+      int stage = 0, phase = 0;    // ring position of the next tile
+      int loaded = 0, q_loads = 0;  // tiles, Q pairs so far
+      int turn = 0;                // units handed to the other warps
+      int index = blockIdx.x;
+      bool go = true;
+      for (int asked = 0; go; ++asked) {
+        if (lane == 0) ask_next(smem_u32(&sh.next), smem_u32(&sh.next_full));
+        PrefillWork w;
+        find_work(p, plan, index, w);
+        w.pad_head = pad_head;
+        w.pad_tail = pad_tail;
+        if (w.seq >= 0 || pads) {
+          if (turn >= 2) wait_or_abort(&sh.work_empty[turn & 1], ((turn >> 1) - 1) & 1, abort);
+          if (lane == 0) {
+            sh.work[turn & 1] = w;
+            mbar_arrive(smem_u32(&sh.work_full[turn & 1]));
+          }
+          __syncwarp();
+          ++turn;
+        }
+        const int steps = max(w.steps[0], w.steps[1]);
+        if (steps > 0) {
+          if (q_loads > 0) wait_or_abort(&sh.q_empty, (q_loads - 1) & 1, abort);
+          ++q_loads;
+          if (__any_sync(0xffffffffu, *abort)) break;
+          if (lane == 0) {
+            const uint32_t bar = smem_u32(&sh.q_full);
+            const int n = (w.steps[0] > 0) + (w.steps[1] > 0);
+            mbar_arrive_expect_tx(bar, n * C::kHalves * p.tile_tokens * p.group * 128);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              for (int h = 0; h < C::kHalves && w.steps[i] > 0; ++h)
+                tma_load_tile_3d(tiles + i * C::kTileBytes + h * C::kHalfBytes, &q_map, h * 64, w.head * p.group,
+                                 w.row0 + w.token0 + i * p.tile_tokens, bar);
+          }
+          __syncwarp();
         }
         for (int t = 0; t < 2 * steps; ++t) {
-          const int stage = t % C::kStages;
-          if (t >= C::kStages) {
-            wait_or_abort(&sh.kv_empty[stage], (t / C::kStages - 1) & 1, abort);
+          if (loaded >= S) {
+            wait_or_abort(&sh.kv_empty[stage], phase ^ 1, abort);
             if (__any_sync(0xffffffffu, *abort)) break;
           }
-          const int key0 = (t >> 1) * kTile;
+          const int tile = w.first + (t >> 1);
           const uint32_t bar = smem_u32(&sh.kv_full[stage]);
           const CUtensorMap* map = (t & 1) ? &v_map : &k_map;
           if (lane == 0) {
             mbar_arrive_expect_tx(bar, C::kTileBytes);
-            if ((t & 1) && (t >> 1) >= open_keys / kTile) mbar_arrive(smem_u32(&sh.v_turn[stage]));
+            if ((t & 1) && tile >= w.open_keys / kTile) mbar_arrive(smem_u32(&sh.v_turn[stage]));
           }
           __syncwarp();
           if (lane < boxes) {
-            const int key = key0 + lane * box_rows;
+            const int key = tile * kTile + lane * box_rows;
             const uint32_t dst = ring + stage * C::kTileBytes + lane * box_rows * 128;
             int page = -1;  // outside the pool: reads as zeros
             if (p.paged && key < w.keys) {
@@ -311,255 +464,324 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
             }
           }
           __syncwarp();
+          ++loaded;
+          if (++stage == S) stage = 0, phase ^= 1;
         }
+        wait_or_abort(&sh.next_full, asked & 1, abort);
+        if (__any_sync(0xffffffffu, *abort)) break;
+        go = answer_next(smem_u32(&sh.next), index);
+        __syncwarp();
       }
+      if (turn >= 2) wait_or_abort(&sh.work_empty[turn & 1], ((turn >> 1) - 1) & 1, abort);
+      if (lane == 0) {
+        sh.work[turn & 1].seq = -2;
+        mbar_arrive(smem_u32(&sh.work_full[turn & 1]));
+      }
+      __syncwarp();
+      // every arrival on this CTA's barriers has to come before it is gone
+      for (int s = 0; s < S && s < loaded; ++s) {
+        if (stage == 0) stage = S, phase ^= 1;
+        --stage;
+        wait_or_abort(&sh.kv_empty[stage], phase, abort);
+      }
+      if (q_loads > 0) wait_or_abort(&sh.q_empty, (q_loads - 1) & 1, abort);
     } else if (warp == 9) {
       // ------------------------------------------------------------ products
       // The whole warp runs the loop, so that the compiler sees uniform values
       // (descriptors in uniform registers); one lane issues.  With the loop in
       // one lane's branch an MMA took 65 cycles to issue, and the issue was
       // what bounded the kernel (567 us for 8192 tokens, 32/8 heads, D 128).
-      if (steps > 0) {
-        constexpr uint64_t k_major = smem_desc_base(16, 1024);
-        constexpr uint64_t v_major = smem_desc_base(C::kHalfBytes, 1024);
-        constexpr uint32_t qk_idesc = mma_idesc(kTile, kTile, false);
-        constexpr uint32_t pv_idesc = mma_idesc(kTile, D, true);
-        const auto qk = [&](int i, int stage) {
-          const uint64_t a = smem_desc(k_major, tiles + i * C::kTileBytes);
-          const uint64_t b = smem_desc(k_major, ring + stage * C::kTileBytes);
-          if (elect_one()) {
+      constexpr uint64_t k_major = smem_desc_base(16, 1024);
+      constexpr uint64_t v_major = smem_desc_base(C::kHalfBytes, 1024);
+      constexpr uint32_t qk_idesc = mma_idesc(kTile, kTile, false);
+      constexpr uint32_t pv_idesc = mma_idesc(kTile, D, true);
+      const auto qk = [&](int i, int stage) {
+        const uint64_t a = smem_desc(k_major, tiles + i * C::kTileBytes);
+        const uint64_t b = smem_desc(k_major, ring + stage * C::kTileBytes);
+        if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              const uint32_t at = ((k >> 2) * C::kHalfBytes + (k & 3) * 32) >> 4;
-              mma_ss(tmem + i * kTile, a + at, b + at, qk_idesc, k > 0);
-            }
-            mma_commit(smem_u32(&sh.s_full[i]));
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t at = ((k >> 2) * C::kHalfBytes + (k & 3) * 32) >> 4;
+            mma_ss(tmem + i * kTile, a + at, b + at, qk_idesc, k > 0);
           }
-          __syncwarp();
-        };
-        const auto pv = [&](int i, int stage, int first, int last, bool accumulate) {
-          const uint64_t v = smem_desc(v_major, ring + stage * C::kTileBytes);
-          if (elect_one()) {
-#pragma unroll
-            for (int k = first; k < last; ++k)
-              mma_ts(tmem + 2 * kTile + i * kTile, tmem + i * kTile + k * 8, v + k * (2048 >> 4), pv_idesc,
-                     accumulate || k > 0);
-          }
-          __syncwarp();
-        };
-        const auto release = [&](int t) {
-          // (no arrival that nobody waits for: it could come after the CTA is gone)
-          if (t + C::kStages < 2 * steps && elect_one()) mma_commit(smem_u32(&sh.kv_empty[t % C::kStages]));
-          __syncwarp();
-        };
-        const int first_open = open_keys / kTile;
-        wait_or_abort(&sh.q_full, 0, abort);
-        wait_or_abort(&sh.kv_full[0], 0, abort);
-        tcgen05_after_sync();
-        if (steps0 > 0) qk(0, 0);
-        if (steps1 > 0) qk(1, 0);
-        release(0);
-        int v_stage = 1, k_stage = 2, v_phase = 0, k_phase = 0;
-        for (int j = 0; j < steps; ++j) {
-          wait_or_abort(&sh.kv_full[v_stage], v_phase, abort);
-          if (j >= first_open) wait_or_abort(&sh.v_clean[v_stage], ((j - first_open) / C::kVPeriod) & 1, abort);
-          if (j + 1 < steps) wait_or_abort(&sh.kv_full[k_stage], k_phase, abort);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int mine = i ? steps1 : steps0;
-            if (j >= mine) continue;
-            wait_or_abort(&sh.p_part[i], j & 1, abort);
-            tcgen05_after_sync();
-            pv(i, v_stage, 0, kFirstPart / 16, j > 0);
-            wait_or_abort(&sh.p_full[i], j & 1, abort);
-            tcgen05_after_sync();
-            pv(i, v_stage, kFirstPart / 16, kTile / 16, true);
-            if (j + 1 < mine) {
-              qk(i, k_stage);
-            } else if (elect_one()) {
-              mma_commit(smem_u32(&sh.o_full[i]));
-            }
-            __syncwarp();
-          }
-          release(2 * j + 1);
-          release(2 * j + 2);
-          v_stage += 2, k_stage += 2;
-          if (v_stage >= C::kStages) v_stage -= C::kStages, v_phase ^= 1;
-          if (k_stage >= C::kStages) k_stage -= C::kStages, k_phase ^= 1;
+          mma_commit(smem_u32(&sh.s_full[i]));
         }
+        __syncwarp();
+      };
+      const auto pv = [&](int i, int stage, int first, int last, bool accumulate) {
+        const uint64_t v = smem_desc(v_major, ring + stage * C::kTileBytes);
+        if (elect_one()) {
+#pragma unroll
+          for (int k = first; k < last; ++k)
+            mma_ts(tmem + 2 * kTile + i * kTile, tmem + i * kTile + k * 8, v + k * (2048 >> 4), pv_idesc,
+                   accumulate || k > 0);
+        }
+        __syncwarp();
+      };
+      const auto commit = [&](uint64_t* bar) {
+        if (elect_one()) mma_commit(smem_u32(bar));
+        __syncwarp();
+      };
+      int stage = 0, phase = 0, q_phase = 0, p_phase0 = 0, p_phase1 = 0;
+      uint32_t clean_phases = 0;  // bit s: parity of v_clean[s]
+      const auto advance = [&] {
+        if (++stage == S) stage = 0, phase ^= 1;
+      };
+      for (int n = 0;; ++n) {
+        if (!next_work(n)) break;
+        const int steps0 = sh.work[n & 1].steps[0], steps1 = sh.work[n & 1].steps[1], steps = max(steps0, steps1);
+        if (steps > 0) {
+          const int first_open = sh.work[n & 1].open_keys / kTile - sh.work[n & 1].first;
+          wait_or_abort(&sh.q_full, q_phase, abort);
+          q_phase ^= 1;
+          wait_or_abort(&sh.kv_full[stage], phase, abort);
+          tcgen05_after_sync();
+          if (steps0 > 0) qk(0, stage);
+          if (steps1 > 0) qk(1, stage);
+          commit(&sh.kv_empty[stage]);
+          if (steps == 1) commit(&sh.q_empty);
+          advance();
+          for (int j = 0; j < steps; ++j) {
+            const int v_stage = stage;
+            wait_or_abort(&sh.kv_full[stage], phase, abort);
+            if (j >= first_open) {
+              wait_or_abort(&sh.v_clean[stage], (clean_phases >> stage) & 1, abort);
+              clean_phases ^= 1u << stage;
+            }
+            advance();
+            const int k_stage = stage;
+            if (j + 1 < steps) {
+              wait_or_abort(&sh.kv_full[stage], phase, abort);
+              advance();
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int mine = i ? steps1 : steps0;
+              if (j >= mine) continue;
+              int& p_phase = i ? p_phase1 : p_phase0;
+              wait_or_abort(&sh.p_part[i], p_phase, abort);
+              tcgen05_after_sync();
+              pv(i, v_stage, 0, kFirstPart / 16, j > 0);
+              wait_or_abort(&sh.p_full[i], p_phase, abort);
+              tcgen05_after_sync();
+              p_phase ^= 1;
+              pv(i, v_stage, kFirstPart / 16, kTile / 16, true);
+              if (j + 1 < mine)
+                qk(i, k_stage);
+              else
+                commit(&sh.o_full[i]);
+            }
+            commit(&sh.kv_empty[v_stage]);
+            if (j + 1 < steps) commit(&sh.kv_empty[k_stage]);
+            if (j + 2 == steps) commit(&sh.q_empty);
+          }
+        }
+        work_done(n);
       }
     } else {
       // ------------------------------------------------------------ masked V
       // Warps 10 and 11 take every other 128 vectors of 16 bytes.
-      bool fix = false;
-      for (int j = open_keys / kTile; j < steps; ++j) {
-        const int t = 2 * j + 1;
-        // the loads' word that the stage has come to tile t, whose parity then is unmistakable
-        wait_or_abort(&sh.v_turn[t % C::kStages], ((j - open_keys / kTile) / C::kVPeriod) & 1, abort);
-        wait_or_abort(&sh.kv_full[t % C::kStages], (t / C::kStages) & 1, abort);
-        const int first = 8 * max(open_keys - j * kTile, 0);            // first vector that some row may not see
-        const int behind = 8 * clamp_to(w.keys - j * kTile, 0, kTile);  // first vector behind the sequence
-        for (int h = 0; h < C::kHalves; ++h) {
-          const uint32_t base = ring + (t % C::kStages) * C::kTileBytes + h * C::kHalfBytes;
-          for (int x0 = (warp - 10) * 128 + lane; x0 < kTile * 8; x0 += 256) {
-            uint4 v[4];
-            uint32_t bad = 0;
+      uint32_t turn_phases = 0;
+      int stage = 0, phase = 0;
+      for (int n = 0;; ++n) {
+        if (!next_work(n)) break;
+        const int steps = max(sh.work[n & 1].steps[0], sh.work[n & 1].steps[1]);
+        const int first_tile = sh.work[n & 1].first, open_keys = sh.work[n & 1].open_keys, keys = sh.work[n & 1].keys;
+        bool fix = false;
+        for (int j = 0; j < steps; ++j) {
+          const int tile = first_tile + j;
+          // past K to V
+          if (++stage == S) stage = 0, phase ^= 1;
+          if (tile >= open_keys / kTile) {
+            // the loads' word that the stage has come to this tile, whose parity then is unmistakable
+            wait_or_abort(&sh.v_turn[stage], (turn_phases >> stage) & 1, abort);
+            turn_phases ^= 1u << stage;
+            wait_or_abort(&sh.kv_full[stage], phase, abort);
+            const int first = 8 * max(open_keys - tile * kTile, 0);           // first vector that some row may not see
+            const int behind = 8 * clamp_to(keys - tile * kTile, 0, kTile);  // first vector behind the sequence
+            for (int h = 0; h < C::kHalves; ++h) {
+              const uint32_t base = ring + stage * C::kTileBytes + h * C::kHalfBytes;
+              for (int x0 = (warp - 10) * 128 + lane; x0 < kTile * 8; x0 += 256) {
+                uint4 v[4];
+                uint32_t bad = 0;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const int x = x0 + 32 * u;
-              v[u] = make_uint4(0, 0, 0, 0);
-              if (x >= first && x < behind) v[u] = ld_shared_v4(base + x * 16);
-            }
+                for (int u = 0; u < 4; ++u) {
+                  const int x = x0 + 32 * u;
+                  v[u] = make_uint4(0, 0, 0, 0);
+                  if (x >= first && x < behind) v[u] = ld_shared_v4(base + x * 16);
+                }
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-              bad |= non_finite_bits(v[u].x) | non_finite_bits(v[u].y) | non_finite_bits(v[u].z) | non_finite_bits(v[u].w);
-            if (bad != 0) {
-              fix = true;
+                for (int u = 0; u < 4; ++u)
+                  bad |= non_finite_bits(v[u].x) | non_finite_bits(v[u].y) | non_finite_bits(v[u].z) |
+                         non_finite_bits(v[u].w);
+                if (bad != 0) {
+                  fix = true;
 #pragma unroll
-              for (int u = 0; u < 4; ++u) {
-                const int x = x0 + 32 * u;
-                if (x >= first && x < behind)
-                  st_shared_v4(base + x * 16, make_uint4(finite_or_zero(v[u].x), finite_or_zero(v[u].y),
-                                                         finite_or_zero(v[u].z), finite_or_zero(v[u].w)));
+                  for (int u = 0; u < 4; ++u) {
+                    const int x = x0 + 32 * u;
+                    if (x >= first && x < behind)
+                      st_shared_v4(base + x * 16, make_uint4(finite_or_zero(v[u].x), finite_or_zero(v[u].y),
+                                                             finite_or_zero(v[u].z), finite_or_zero(v[u].w)));
+                  }
+                }
+                if (x0 + 96 >= behind) {
+#pragma unroll
+                  for (int u = 0; u < 4; ++u)
+                    if (x0 + 32 * u >= behind) st_shared_v4(base + (x0 + 32 * u) * 16, make_uint4(0, 0, 0, 0));
+                }
               }
             }
-            if (x0 + 96 >= behind) {
-#pragma unroll
-              for (int u = 0; u < 4; ++u)
-                if (x0 + 32 * u >= behind) st_shared_v4(base + (x0 + 32 * u) * 16, make_uint4(0, 0, 0, 0));
-            }
+            fence_proxy_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sh.v_clean[stage]));
           }
+          if (++stage == S) stage = 0, phase ^= 1;
         }
-        fence_proxy_async_shared();
+        if (fix) *reinterpret_cast<volatile int*>(&sh.fix[n & 1]) = n + 1;
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.v_clean[t % C::kStages]));
+        if (lane == 0) mbar_arrive(smem_u32(&sh.fix_done[n & 1]));
+        work_done(n);
       }
-      if (fix) *reinterpret_cast<volatile int*>(&sh.fix) = 1;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh.fix_done));
     }
   } else {
     // ------------------------------------------------------------ softmax
     regs_inc<kSoftmaxRegs>();
     const int i = warp >> 2;
-    const int mine = i ? steps1 : steps0;
     const int row = tid & (kTile - 1);
-    const int valid = w.seq < 0 ? 0 : tile_valid(p, w, i);
-    const int token = row / p.group;
-    const bool live = row < p.tile_tokens * p.group && token < valid;
-    const int t = w.token0 + i * p.tile_tokens + token;
-    const int sees = live ? keys_of(w, t) : 0;
-    const int all_see = keys_of(w, w.token0 + i * p.tile_tokens);  // keys that every row of the tile sees
+    const int token = row / p.group, member = row - token * p.group;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + i * kTile + lanes, o_at = tmem + 2 * kTile + i * kTile + lanes;
     const float scale = p.scale_log2;
-    float top = -INFINITY, total = 0.f;
-    for (int j = 0; j < mine; ++j) {
-      wait_or_abort(&sh.s_full[i], j & 1, abort);
-      tcgen05_after_sync();
-      float s[kTile];
-#pragma unroll
-      for (int c = 0; c < kTile; c += 32) tmem_ld32(s_at + c, s + c);
-      tmem_wait_ld();
-      if ((j + 1) * kTile > all_see) {
-        const int limit = sees - j * kTile;
-#pragma unroll
-        for (int c = 0; c < kTile; ++c) s[c] = c < limit ? s[c] : -INFINITY;
+    int s_phase = 0, o_phase = 0;
+    for (int n = 0;; ++n) {
+      if (!next_work(n)) break;
+      const PrefillWork& w = sh.work[n & 1];
+      if (w.pad_tail < p.total || w.pad_head > 0) {
+        const int64_t vecs = static_cast<int64_t>(p.q_heads) * (D / 8);
+        uint4* o = reinterpret_cast<uint4*>(p.out);
+        const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+        const int64_t at = static_cast<int64_t>(w.index) * 256 + tid;
+        for (int64_t x = w.pad_tail * vecs + at; x < p.total * vecs; x += step) o[x] = make_uint4(0, 0, 0, 0);
+        for (int64_t x = at; x < w.pad_head * vecs; x += step) o[x] = make_uint4(0, 0, 0, 0);
       }
-      float m0 = -INFINITY, m1 = m0, m2 = m0, m3 = m0;
+      const int steps = i ? w.steps[1] : w.steps[0], valid = i ? w.valid[1] : w.valid[0];
+      const bool live = token < valid;
+      // keys that the row sees, and that every row of the tile sees, from the unit's first on
+      const int all_see = keys_of(w, w.token0 + i * p.tile_tokens) - w.first * kTile;
+      const int sees = live ? all_see + token : 0;
+      float top = -INFINITY, total = 0.f;
+      for (int j = 0; j < steps; ++j) {
+        wait_or_abort(&sh.s_full[i], s_phase, abort);
+        s_phase ^= 1;
+        tcgen05_after_sync();
+        float s[kTile];
 #pragma unroll
-      for (int c = 0; c < kTile; c += 8) {
-        m0 = max3(m0, s[c], s[c + 1]);
-        m1 = max3(m1, s[c + 2], s[c + 3]);
-        m2 = max3(m2, s[c + 4], s[c + 5]);
-        m3 = max3(m3, s[c + 6], s[c + 7]);
+        for (int c = 0; c < kTile; c += 32) tmem_ld32(s_at + c, s + c);
+        tmem_wait_ld();
+        if ((j + 1) * kTile > all_see) {
+          const int limit = sees - j * kTile;
+#pragma unroll
+          for (int c = 0; c < kTile; ++c) s[c] = c < limit ? s[c] : -INFINITY;
+        }
+        float m0 = -INFINITY, m1 = m0, m2 = m0, m3 = m0;
+#pragma unroll
+        for (int c = 0; c < kTile; c += 8) {
+          m0 = max3(m0, s[c], s[c + 1]);
+          m1 = max3(m1, s[c + 2], s[c + 3]);
+          m2 = max3(m2, s[c + 4], s[c + 5]);
+          m3 = max3(m3, s[c + 6], s[c + 7]);
+        }
+        const float high = fmaxf(max3(m0, m1, m2), m3);
+        if (j == 0) {
+          top = high;
+        } else if (__any_sync(0xffffffffu, live && (high - top) * scale > kRescaleLog2)) {
+          // O_i holds the sum up to tile j - 1: S_i was issued after that product.  Rows outside the
+          // sequence have no say: the result would depend on what lies there.
+          const float next = fmaxf(top, high);
+          const float keep = next == top ? 1.f : fast_exp2((top - next) * scale);
+          top = next;
+          total *= keep;
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {  // few registers: S is still in hand
+            uint32_t o[16];
+            tmem_ld16(o_at + c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+            tmem_st16(o_at + c, o);
+          }
+        }
+        const float shift = top == -INFINITY ? 0.f : -top * scale;
+        const uint64_t scale2 = pack2(scale, scale), shift2 = pack2(shift, shift);
+        uint64_t sum0 = 0, sum1 = 0;
+#pragma unroll
+        for (int c = 0; c < kTile; c += 32) {
+          uint32_t w16[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float a, b;
+            unpack2(fma2(pack2(s[c + 2 * e], s[c + 2 * e + 1]), scale2, shift2), a, b);
+            a = fast_exp2(a);
+            b = fast_exp2(b);
+            if (e & 1)
+              sum1 = add2(sum1, pack2(a, b));
+            else
+              sum0 = add2(sum0, pack2(a, b));
+            w16[e] = pack_bf16x2(a, b);
+          }
+          tmem_st16(s_at + c / 2, w16);
+          if (c + 32 == kFirstPart) {
+            tmem_wait_st();
+            tcgen05_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sh.p_part[i]));
+          }
+        }
+        tmem_wait_st();
+        tcgen05_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[i]));
+        float a, b;
+        unpack2(add2(sum0, sum1), a, b);
+        total += a + b;
       }
-      const float high = fmaxf(max3(m0, m1, m2), m3);
-      if (j == 0) {
-        top = high;
-      } else if (__any_sync(0xffffffffu, live && (high - top) * scale > kRescaleLog2)) {
-        // O_i holds the sum up to tile j - 1: S_i was issued after that product.  Rows outside the
-        // sequence have no say: the result would depend on what lies there.
-        const float next = fmaxf(top, high);
-        const float keep = next == top ? 1.f : fast_exp2((top - next) * scale);
-        top = next;
-        total *= keep;
-#pragma unroll
+      wait_or_abort(&sh.fix_done[n & 1], (n >> 1) & 1, abort);
+      if (steps > 0) {
+        wait_or_abort(&sh.o_full[i], o_phase, abort);
+        o_phase ^= 1;
+        tcgen05_after_sync();
+      }
+      if (__any_sync(0xffffffffu, *abort)) break;
+      const float inv = total == 0.f ? 0.f : 1.f / total;
+      const int t = w.token0 + i * p.tile_tokens + token;
+      __nv_bfloat16* out = p.out + (static_cast<int64_t>(w.row0 + t) * p.q_heads + w.head * p.group + member) * D;
+      if (valid > 0) {
+#pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           float o[32];
-          tmem_ld32(o_at + c, o);
-          tmem_wait_ld();
+          if (steps > 0) {
+            tmem_ld32(o_at + c, o);
+            tmem_wait_ld();
+          }
+          uint32_t x[16];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] *= keep;
-          tmem_st32(o_at + c, o);
+          for (int e = 0; e < 16; ++e) {
+            const float a = inv == 0.f ? 0.f : o[2 * e] * inv, b = inv == 0.f ? 0.f : o[2 * e + 1] * inv;
+            x[e] = pack_bf16x2(a, b);
+          }
+          if (live) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<uint4*>(out + c + e * 8) =
+                  make_uint4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+          }
         }
+        if (live && *reinterpret_cast<volatile int*>(&sh.fix[n & 1]) == n + 1)
+          add_non_finite(p, w.seq, w.head, w.row0, D, w.open_keys, keys_of(w, t), out);
       }
-      const float shift = top == -INFINITY ? 0.f : -top * scale;
-      const uint64_t scale2 = pack2(scale, scale), shift2 = pack2(shift, shift);
-      uint64_t sum0 = 0, sum1 = 0;
-#pragma unroll
-      for (int c = 0; c < kTile; c += 32) {
-        uint32_t w16[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float a, b;
-          unpack2(fma2(pack2(s[c + 2 * e], s[c + 2 * e + 1]), scale2, shift2), a, b);
-          a = fast_exp2(a);
-          b = fast_exp2(b);
-          if (e & 1)
-            sum1 = add2(sum1, pack2(a, b));
-          else
-            sum0 = add2(sum0, pack2(a, b));
-          w16[e] = pack_bf16x2(a, b);
-        }
-        tmem_st16(s_at + c / 2, w16);
-        if (c + 32 == kFirstPart) {
-          tmem_wait_st();
-          tcgen05_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&sh.p_part[i]));
-        }
-      }
-      tmem_wait_st();
       tcgen05_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[i]));
-      float a, b;
-      unpack2(add2(sum0, sum1), a, b);
-      total += a + b;
+      work_done(n);
     }
-    if (mine > 0) {
-      wait_or_abort(&sh.fix_done, 0, abort);
-      wait_or_abort(&sh.o_full[i], 0, abort);
-      tcgen05_after_sync();
-    }
-    const bool ok = __all_sync(0xffffffffu, *abort == 0);
-    const float inv = mine == 0 || total == 0.f ? 0.f : 1.f / total;
-    __nv_bfloat16* out = p.out + (static_cast<int64_t>(w.row0 + t) * p.q_heads + w.head * p.group + row % p.group) * D;
-    if (ok && valid > 0) {
-#pragma unroll 1
-      for (int c = 0; c < D; c += 32) {
-        float o[32];
-        if (mine > 0) {
-          tmem_ld32(o_at + c, o);
-          tmem_wait_ld();
-        }
-        uint32_t x[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float a = inv == 0.f ? 0.f : o[2 * e] * inv, b = inv == 0.f ? 0.f : o[2 * e + 1] * inv;
-          x[e] = pack_bf16x2(a, b);
-        }
-        if (live) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<uint4*>(out + c + e * 8) = make_uint4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
-        }
-      }
-    }
-    if (ok && live && *reinterpret_cast<volatile int*>(&sh.fix) != 0)
-      add_non_finite(p, w.seq, w.head, w.row0, D, open_keys, sees, out);
-    tcgen05_before_sync();
   }
   __syncthreads();
   griddep_launch_dependents();

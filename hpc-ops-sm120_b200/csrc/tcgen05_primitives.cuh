@@ -44,16 +44,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float* r) {
       : "memory");
 }
 
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const float* r) {
-  const uint32_t* u = reinterpret_cast<const uint32_t*>(r);
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* u) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
-      "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
-      "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]),
-      "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]),
-      "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+      : "r"(addr)
       : "memory");
 }
 
@@ -133,6 +130,35 @@ __device__ __forceinline__ void tma_load_tile_4d(uint32_t dst, const CUtensorMap
       "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
       : "memory");
+}
+
+// ---------------------------------------------------------------- launch control
+// Asks for the index of a CTA of this grid that has not started; the 16-byte
+// answer at `dst` completes on `bar`.  Not to be asked again after a refusal.
+__device__ __forceinline__ void ask_next(uint32_t dst, uint32_t bar) {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  mbar_arrive_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   dst),
+               "r"(bar)
+               : "memory");
+}
+
+// Whether there was one, and its index (x).
+__device__ __forceinline__ bool answer_next(uint32_t src, int& index) {
+  uint32_t yes, x;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 h;\n\t"
+      "ld.shared.b128 h, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+      : "=r"(yes), "=r"(x)
+      : "r"(src)
+      : "memory");
+  if (yes) index = static_cast<int>(x);
+  return yes != 0;
 }
 
 // ---------------------------------------------------------------- registers
