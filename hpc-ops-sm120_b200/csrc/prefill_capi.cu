@@ -123,6 +123,7 @@ int launch(adb::PrefillParams& p, const void* q, int64_t q_token, int64_t q_head
   if (rc != ADB_OK) return rc;
   p.scale_log2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(dim)));
   p.tile_tokens = adb::kTile / p.group;
+  p.group_magic = (65536 + p.group - 1) / p.group;
   CUtensorMap q_map, k_map, v_map;
   rc = encode_packed(&q_map, q, p.total, p.q_heads, dim, q_token, q_head, p.group, p.tile_tokens);
   if (rc != ADB_OK) return rc;

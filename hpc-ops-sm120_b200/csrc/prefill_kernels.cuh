@@ -62,6 +62,7 @@ struct PrefillParams {
   int total, batch, q_heads, kv_heads, group;
   int tile_tokens;         // tokens of a Q tile: 128 / group
   int head_group;          // KV heads that are worked on at a time
+  int group_magic;         // ceil(2^16 / group): row / group = row * magic >> 16 for rows below 128
   int paged;               // 0 packed K/V, 1 HND pages, 2 NHD pages
   int max_blocks, num_blocks, page_shift;
   float scale_log2;        // log2(e) / sqrt(D)
@@ -72,8 +73,8 @@ struct PrefillCfg {
   static constexpr int kHalves = D / 64;                     // 128-byte column blocks of a row
   static constexpr int kHalfBytes = kTile * 128;             // one column block of a tile
   static constexpr int kTileBytes = kHalves * kHalfBytes;
-  static constexpr int kStages = D == 128 ? 5 : 8;           // K and V tiles in flight
-  static constexpr int kSmemBytes = (2 + kStages) * kTileBytes + 1024;
+  static constexpr int kStages = D == 128 ? 4 : 8;           // K and V tiles in flight
+  static constexpr int kSmemBytes = (2 + kStages) * kTileBytes + 2 * kHalfBytes + 1024;
 };
 
 // What a CTA works on.
@@ -136,21 +137,28 @@ __device__ __forceinline__ int sequence_keys(const PrefillParams& p, int b, int 
   return p.paged ? clamp_to(p.lens[b], 0, p.max_blocks << p.page_shift) : count;
 }
 
+__device__ __forceinline__ int pairs_of(const PrefillParams& p, int count) {
+  return static_cast<int>(static_cast<unsigned>(count + 2 * p.tile_tokens - 1) / static_cast<unsigned>(2 * p.tile_tokens));
+}
+
 __device__ __forceinline__ void make_plan(const PrefillParams& p, PrefillPlan& plan) {
   const int lane = threadIdx.x & 31;
-  const int per = 2 * p.tile_tokens;
   plan.scan_base = plan.scan_before = 0;
   int units = 0, top = 0;
+#pragma unroll
+  for (int r = 0; r < kPlanRows; ++r) plan.pairs[r] = plan.base[r] = 0;
   if (plan_is_sorted(p)) {
 #pragma unroll
     for (int r = 0; r < kPlanRows; ++r) {
-      plan.pairs[r] = plan.base[r] = 0;
+      if (32 * r >= p.batch) break;
       const int b = 32 * r + lane;
       if (b < p.batch) {
         int first, count;
         sequence_rows(p, b, first, count);
-        plan.pairs[r] = (count + per - 1) / per;
-        plan.base[r] = max(sequence_keys(p, b, count) - count, 0) / per;
+        plan.pairs[r] = pairs_of(p, count);
+        if (p.paged)
+          plan.base[r] = static_cast<int>(static_cast<unsigned>(max(sequence_keys(p, b, count) - count, 0)) /
+                                          static_cast<unsigned>(2 * p.tile_tokens));
         units += plan.pairs[r];
         top = max(top, plan.base[r] + plan.pairs[r]);
       }
@@ -159,7 +167,7 @@ __device__ __forceinline__ void make_plan(const PrefillParams& p, PrefillPlan& p
     for (int b = lane; b < p.batch; b += 32) {
       int first, count;
       sequence_rows(p, b, first, count);
-      units += (count + per - 1) / per;
+      units += pairs_of(p, count);
     }
   }
   plan.units = __reduce_add_sync(0xffffffffu, units);
@@ -180,6 +188,11 @@ __device__ __forceinline__ int warp_prefix(int v) {
 // Sequence and pair of the r-th unit of the plan (r < units).
 __device__ __forceinline__ void find_pair(const PrefillParams& p, PrefillPlan& plan, int r, int& seq, int& pair) {
   const int lane = threadIdx.x & 31;
+  if (p.batch == 1) {
+    seq = 0;
+    pair = plan.units - 1 - r;
+    return;
+  }
   if (plan_is_sorted(p)) {
     // lowest level with at most r pairs above it
     int lo = 0, hi = plan.top, above = 0;
@@ -187,7 +200,10 @@ __device__ __forceinline__ void find_pair(const PrefillParams& p, PrefillPlan& p
       const int mid = (lo + hi) >> 1;
       int n = 0;
 #pragma unroll
-      for (int s = 0; s < kPlanRows; ++s) n += clamp_to(plan.base[s] + plan.pairs[s] - mid, 0, plan.pairs[s]);
+      for (int s = 0; s < kPlanRows; ++s) {
+        if (32 * s >= p.batch) break;
+        n += clamp_to(plan.base[s] + plan.pairs[s] - mid, 0, plan.pairs[s]);
+      }
       n = __reduce_add_sync(0xffffffffu, n);
       if (n <= r)
         hi = mid, above = n;
@@ -196,30 +212,28 @@ __device__ __forceinline__ void find_pair(const PrefillParams& p, PrefillPlan& p
     }
     int k = r - above;
     seq = pair = 0;
-    bool found = false;
 #pragma unroll
     for (int s = 0; s < kPlanRows; ++s) {
       const bool here = plan.base[s] < hi && hi <= plan.base[s] + plan.pairs[s];
       const unsigned all = __ballot_sync(0xffffffffu, here);
       const int n = __popc(all);
-      if (!found && k < n) {
-        found = true;
+      if (k < n) {
         const unsigned mine = __ballot_sync(0xffffffffu, here && __popc(all & ((1u << lane) - 1)) == k);
         const int l = __ffs(mine) - 1;
         seq = 32 * s + l;
         pair = hi - __shfl_sync(0xffffffffu, plan.base[s], l) - 1;
+        break;
       }
       k -= n;
     }
     return;
   }
-  const int per = 2 * p.tile_tokens;
   if (r < plan.scan_before) plan.scan_base = plan.scan_before = 0;
   for (;;) {
     const int b = plan.scan_base + lane;
     int first = 0, count = 0;
     if (b < p.batch) sequence_rows(p, b, first, count);
-    const int mine = (count + per - 1) / per;
+    const int mine = pairs_of(p, count);
     const int inc = warp_prefix(mine);
     const unsigned hit = __ballot_sync(0xffffffffu, r < plan.scan_before + inc);
     if (hit) {
@@ -333,6 +347,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const uint32_t tiles = (smem_u32(raw) + 1023u) & ~1023u;  // Q_0 Q_1, then the K/V ring
   const uint32_t ring = tiles + 2 * C::kTileBytes;
+  const uint32_t staging = ring + S * C::kTileBytes;  // 64 columns of each output tile
   volatile int* abort = &sh.abort;
 
   if (tid == 0) {
@@ -386,9 +401,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     regs_dec<kOtherRegs>();
     if (warp == 8) {
       // ------------------------------------------------------------ loads
+      const int pad_tail = clamp_to(p.cu[p.batch], 0, p.total), pad_head = clamp_to(p.cu[0], 0, p.total);
       PrefillPlan plan;
       make_plan(p, plan);
-      const int pad_tail = clamp_to(p.cu[p.batch], 0, p.total), pad_head = clamp_to(p.cu[0], 0, p.total);
       const bool pads = pad_tail < p.total || pad_head > 0;
       const int boxes = p.paged ? max(1, kTile >> p.page_shift) : 1;
       const int box_rows = kTile / boxes;
@@ -648,7 +663,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     regs_inc<kSoftmaxRegs>();
     const int i = warp >> 2;
     const int row = tid & (kTile - 1);
-    const int token = row / p.group, member = row - token * p.group;
+    const int token = row * p.group_magic >> 16;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + i * kTile + lanes, o_at = tmem + 2 * kTile + i * kTile + lanes;
     const float scale = p.scale_log2;
@@ -752,32 +767,45 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         tcgen05_after_sync();
       }
       if (__any_sync(0xffffffffu, *abort)) break;
+      // A warp's 32 rows go through shared memory, 64 columns at a time, so that a
+      // store covers whole lines (16 bytes of 32 rows each took 2.5 us per unit).
       const float inv = total == 0.f ? 0.f : 1.f / total;
-      const int t = w.token0 + i * p.tile_tokens + token;
-      __nv_bfloat16* out = p.out + (static_cast<int64_t>(w.row0 + t) * p.q_heads + w.head * p.group + member) * D;
-      if (valid > 0) {
+      __nv_bfloat16* out = p.out + (static_cast<int64_t>(w.row0 + w.token0 + i * p.tile_tokens) * p.q_heads +
+                                    w.head * p.group) * D;
+      const int64_t gap = static_cast<int64_t>(p.q_heads - p.group) * D;  // between the rows of two tokens
+      const int rows = valid * p.group;
+      const uint32_t mine = staging + i * C::kHalfBytes + (warp & 3) * 4096;
+      if ((warp & 3) * 32 < rows) {
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          float o[32];
-          if (steps > 0) {
-            tmem_ld32(o_at + c, o);
-            tmem_wait_ld();
-          }
-          uint32_t x[16];
+        for (int c = 0; c < D; c += 64) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float a = inv == 0.f ? 0.f : o[2 * e] * inv, b = inv == 0.f ? 0.f : o[2 * e + 1] * inv;
-            x[e] = pack_bf16x2(a, b);
-          }
-          if (live) {
+          for (int h = 0; h < 64; h += 32) {
+            float o[32];
+            if (steps > 0) {
+              tmem_ld32(o_at + c + h, o);
+              tmem_wait_ld();
+            }
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = inv == 0.f ? 0.f : o[e] * inv;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              *reinterpret_cast<uint4*>(out + c + e * 8) =
-                  make_uint4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+              st_shared_v4(mine + lane * 128 + (((h >> 3) + e) ^ (lane & 7)) * 16,
+                           make_uint4(pack_bf16x2(o[8 * e], o[8 * e + 1]), pack_bf16x2(o[8 * e + 2], o[8 * e + 3]),
+                                      pack_bf16x2(o[8 * e + 4], o[8 * e + 5]), pack_bf16x2(o[8 * e + 6], o[8 * e + 7])));
           }
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int l = 4 * k + (lane >> 3), x = lane & 7, r = (warp & 3) * 32 + l;
+            const uint4 v = ld_shared_v4(mine + l * 128 + (x ^ (l & 7)) * 16);
+            if (r < rows)
+              *reinterpret_cast<uint4*>(out + (r * p.group_magic >> 16) * gap + static_cast<int64_t>(r) * D + c + x * 8) = v;
+          }
+          __syncwarp();
         }
         if (live && *reinterpret_cast<volatile int*>(&sh.fix[n & 1]) == n + 1)
-          add_non_finite(p, w.seq, w.head, w.row0, D, w.open_keys, keys_of(w, t), out);
+          add_non_finite(p, w.seq, w.head, w.row0, D, w.open_keys, w.first * kTile + sees,
+                         out + token * gap + static_cast<int64_t>(row) * D);
       }
       tcgen05_before_sync();
       work_done(n);
