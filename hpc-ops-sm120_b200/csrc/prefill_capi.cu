@@ -112,9 +112,32 @@ int prepare(int device) {
   return ADB_OK;
 }
 
+size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+// Workspace: the counters (zero between calls), then O and (maximum, total) of
+// the parts.  A part is two thirds of an SM's even share of all K/V tiles or
+// more, and the pairs of a sequence have half its tiles or more on average, so
+// that there are at most three times as many parts as SMs.
+struct Workspace {
+  int64_t slots, rows;
+  size_t header, off_o, off_ml, bytes;
+};
+
+Workspace plan_workspace(int64_t total, int64_t group, int64_t dim, int64_t sms) {
+  Workspace w;
+  w.slots = 3 * sms;
+  w.rows = std::min<int64_t>(2 * (adb::kTile / group), total) * group;
+  w.header = static_cast<size_t>(w.slots) * sizeof(uint32_t);
+  w.off_o = align256(w.header);
+  w.off_ml = w.off_o + static_cast<size_t>(w.slots * w.rows * dim) * sizeof(float);
+  w.bytes = w.off_ml + align256(static_cast<size_t>(w.slots * w.rows) * sizeof(float2));
+  return w;
+}
+
 // `k`, the K tensor; p holds everything else.
 int launch(adb::PrefillParams& p, const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
-           int64_t k_head, int64_t dim, int device, void* stream) {
+           int64_t k_head, int64_t dim, void* workspace, size_t workspace_bytes, unsigned flags, int device,
+           void* stream) {
   DeviceGuard guard(device);
   if (guard.error != cudaSuccess) return cuda_fail(guard.error, "cudaSetDevice");
   int sms = 0;
@@ -138,14 +161,31 @@ int launch(adb::PrefillParams& p, const void* q, int64_t q_token, int64_t q_head
   // every sequence with a token may end in a partly filled pair of tiles
   const int64_t per = 2 * p.tile_tokens;
   const int64_t pairs = p.total / per + std::min(p.batch, p.total);
+  const Workspace ws = plan_workspace(p.total, p.group, dim, sms);
+  if (workspace == nullptr || !is_aligned(workspace, 256))
+    return fail(ADB_ERR_WORKSPACE, "workspace must be a non-null 256-byte aligned device buffer");
+  if (workspace_bytes < ws.bytes)
+    return fail(ADB_ERR_WORKSPACE, "workspace too small: %zu bytes given, %zu needed", workspace_bytes, ws.bytes);
+  uint8_t* base = static_cast<uint8_t*>(workspace);
+  p.sms = sms;
+  p.max_slots = static_cast<int>(ws.slots);
+  p.slot_rows = static_cast<int>(ws.rows);
+  p.counters = reinterpret_cast<uint32_t*>(base);
+  p.part_o = reinterpret_cast<float4*>(base + ws.off_o);
+  p.part_ml = reinterpret_cast<float2*>(base + ws.off_ml);
   // KV heads worked on at a time: as many as keep the longest possible
   // sequence's K and V within half of L2
   const int64_t keys = p.paged ? int64_t(p.max_blocks) << p.page_shift : p.total;
   p.head_group = static_cast<int>(
       std::max<int64_t>(1, std::min<int64_t>(p.kv_heads, kL2Bytes / 2 / std::max<int64_t>(1, keys * dim * 4))));
-  if (pairs * p.kv_heads > INT32_MAX) return fail(ADB_ERR_INVALID_ARGUMENT, "too many tiles for one call");
+  const int64_t grid = pairs * p.kv_heads + ws.slots;
+  if (grid > INT32_MAX) return fail(ADB_ERR_INVALID_ARGUMENT, "too many tiles for one call");
+  if (!(flags & ADB_FLAG_HEADER_ZEROED)) {
+    const cudaError_t me = cudaMemsetAsync(workspace, 0, ws.header, static_cast<cudaStream_t>(stream));
+    if (me != cudaSuccess) return cuda_fail(me, "workspace header memset");
+  }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(pairs * p.kv_heads));
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(adb::kPrefillThreads);
   cfg.dynamicSmemBytes = dim == 128 ? adb::PrefillCfg<128>::kSmemBytes : adb::PrefillCfg<64>::kSmemBytes;
   cfg.stream = static_cast<cudaStream_t>(stream);
@@ -170,9 +210,12 @@ int adb_prefill_workspace_size(int64_t total, int64_t batch, int64_t q_heads, in
   if (bytes == nullptr) return fail(ADB_ERR_INVALID_ARGUMENT, "bytes pointer is null");
   const int rc = check_heads(total, batch, q_heads, kv_heads, head_dim);
   if (rc != ADB_OK) return rc;
-  (void)device;
-  *bytes = 256;
-  if (header_bytes != nullptr) *header_bytes = 0;
+  int sms = 0;
+  const int status = adb_host::sm_count(device, &sms);
+  if (status != ADB_OK) return status;
+  const Workspace w = plan_workspace(total, q_heads / kv_heads, head_dim, sms);
+  *bytes = w.bytes;
+  if (header_bytes != nullptr) *header_bytes = w.header;
   return ADB_OK;
 }
 
@@ -199,7 +242,8 @@ int adb_prefill(const void* q, int64_t q_token_stride, int64_t q_head_stride, co
   p.q_heads = static_cast<int>(q_heads);
   p.kv_heads = static_cast<int>(kv_heads);
   p.group = static_cast<int>(q_heads / kv_heads);
-  return launch(p, q, q_token_stride, q_head_stride, k, k_token_stride, k_head_stride, head_dim, device, stream);
+  return launch(p, q, q_token_stride, q_head_stride, k, k_token_stride, k_head_stride, head_dim, workspace,
+                workspace_bytes, flags, device, stream);
 }
 
 int adb_prefill_paged(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
@@ -246,7 +290,8 @@ int adb_prefill_paged(const void* q, int64_t q_token_stride, int64_t q_head_stri
   p.max_blocks = static_cast<int>(max_blocks_per_seq);
   p.num_blocks = static_cast<int>(num_blocks);
   while ((int64_t(1) << p.page_shift) < page_size) ++p.page_shift;
-  return launch(p, q, q_token_stride, q_head_stride, k_cache, 0, 0, head_dim, device, stream);
+  return launch(p, q, q_token_stride, q_head_stride, k_cache, 0, 0, head_dim, workspace, workspace_bytes, flags,
+                device, stream);
 }
 
 }  // extern "C"

@@ -18,6 +18,12 @@
 // control), so that one CTA's loads and first products overlap the end of its
 // unit before.  Units that see the most keys come first.
 //
+// Splits.  Where a sequence's K/V tiles are one and a half times an SM's even
+// share of all tiles or more (few rows over a long cache), its pairs are cut
+// into parts of about that share.  A part leaves its unnormalised O and (maximum, total) in the
+// workspace; the part of a tile that finishes last joins them, in the order of
+// the parts, so that the result does not depend on which one that is.
+//
 // Pipeline of a CTA (384 threads):
 //   warps 0-3, 4-7   softmax of tile 0, 1: one thread per row
 //   warp 8           finds the units; TMA loads: Q, then K_0 V_0 K_1 V_1 ...
@@ -47,8 +53,9 @@ constexpr int kPrefillThreads = 384;
 constexpr int kTile = 128;  // rows of a Q tile, keys of a K/V tile
 constexpr int kFirstPart = 64;  // keys whose weights are handed to the tensor cores before the others are computed
 constexpr float kRescaleLog2 = 8.f;
+constexpr int kMinPart = 8;     // K/V tiles of a part, at least
 // Registers: 12 warps x 168 at launch; the loading and issuing warps give theirs to the softmax.
-constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
+constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
 static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * 168, "more registers than the block is launched with");
 
 struct PrefillParams {
@@ -66,6 +73,12 @@ struct PrefillParams {
   int paged;               // 0 packed K/V, 1 HND pages, 2 NHD pages
   int max_blocks, num_blocks, page_shift;
   float scale_log2;        // log2(e) / sqrt(D)
+  int sms;
+  int max_slots;           // parts that the workspace holds (0: no splits)
+  int slot_rows;           // rows of a part: group times the tokens of a pair, or of all sequences
+  uint32_t* counters;      // [max_slots] finished parts per tile of a pair, zero between calls
+  float4* part_o;          // [max_slots][D / 4][slot_rows]
+  float2* part_ml;         // [max_slots][slot_rows] maximum (of q . k), total
 };
 
 template <int D>
@@ -89,6 +102,9 @@ struct PrefillWork {
   int first;         // K/V tiles first .. first + steps[i] - 1 are tile i's
   int steps[2];
   int open_keys;     // keys from here on are hidden from some row of the tiles
+  int parts, part;   // of the pair's K/V tiles
+  int slot;          // of the pair's part 0 in the workspace
+  int counter;       // of tile 0
   int pad_head, pad_tail;  // rows before the first / from the end of the last sequence
 };
 
@@ -103,8 +119,10 @@ struct PrefillShared {
   uint64_t v_turn[PrefillCfg<D>::kStages];   // a border tile of V is on its way
   uint64_t v_clean[PrefillCfg<D>::kStages];  // and cleared
   uint64_t fix_done[2];
+  uint64_t tile_sync[2];  // the four warps of a tile
   uint32_t tmem;
   int abort;
+  int last[2];       // this CTA's part of tile i finished last
   int fix[2];        // number of the unit of which a non-finite value of V was cleared
   PrefillWork work[2];
 };
@@ -126,7 +144,8 @@ __device__ __forceinline__ void sequence_rows(const PrefillParams& p, int b, int
 constexpr int kPlanRows = 8;
 struct PrefillPlan {
   int pairs[kPlanRows], base[kPlanRows];
-  int units;                       // pairs of all sequences
+  int parts[kPlanRows];            // of each of a sequence's pairs
+  int units;                       // parts of all pairs of all sequences
   int top;                         // highest level
   int scan_base, scan_before;      // where the walk stands
 };
@@ -145,8 +164,9 @@ __device__ __forceinline__ void make_plan(const PrefillParams& p, PrefillPlan& p
   const int lane = threadIdx.x & 31;
   plan.scan_base = plan.scan_before = 0;
   int units = 0, top = 0;
+  float tiles = 0.f;  // K/V tiles of all pairs
 #pragma unroll
-  for (int r = 0; r < kPlanRows; ++r) plan.pairs[r] = plan.base[r] = 0;
+  for (int r = 0; r < kPlanRows; ++r) plan.pairs[r] = plan.base[r] = 0, plan.parts[r] = 1;
   if (plan_is_sorted(p)) {
 #pragma unroll
     for (int r = 0; r < kPlanRows; ++r) {
@@ -161,6 +181,34 @@ __device__ __forceinline__ void make_plan(const PrefillParams& p, PrefillPlan& p
                                           static_cast<unsigned>(2 * p.tile_tokens));
         units += plan.pairs[r];
         top = max(top, plan.base[r] + plan.pairs[r]);
+        // for now the tiles of the sequence's last pair, its longest
+        const int keys = p.paged ? sequence_keys(p, b, count) : count;
+        plan.parts[r] = (keys + kTile - 1) / kTile;
+        tiles += 0.5f * plan.pairs[r] * (plan.parts[r] + (max(keys - count, 0) + kTile) / kTile);
+      }
+    }
+    // parts of an SM's even share
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, d);
+    int share = max(kMinPart, static_cast<int>(fminf(ceilf(tiles * p.kv_heads / p.sms), 1e9f)));
+    for (bool fits = false; !fits; share *= 2) {
+      float slots = 0.f;
+#pragma unroll
+      for (int r = 0; r < kPlanRows; ++r) {
+        if (32 * r >= p.batch) break;
+        const int parts = (2 * plan.parts[r] + share) / (2 * share);
+        if (parts > 1) slots += static_cast<float>(plan.pairs[r]) * parts;
+      }
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) slots += __shfl_xor_sync(0xffffffffu, slots, d);
+      fits = slots * p.kv_heads <= p.max_slots;
+      if (!fits) continue;
+      units = 0;
+#pragma unroll
+      for (int r = 0; r < kPlanRows; ++r) {
+        if (32 * r >= p.batch) break;
+        plan.parts[r] = max(1, (2 * plan.parts[r] + share) / (2 * share));
+        units += plan.pairs[r] * plan.parts[r];
       }
     }
   } else {
@@ -185,14 +233,12 @@ __device__ __forceinline__ int warp_prefix(int v) {
   return v;
 }
 
-// Sequence and pair of the r-th unit of the plan (r < units).
-__device__ __forceinline__ void find_pair(const PrefillParams& p, PrefillPlan& plan, int r, int& seq, int& pair) {
+// Sequence, pair and part of the r-th unit of the plan (r < units).
+__device__ __forceinline__ void find_pair(const PrefillParams& p, PrefillPlan& plan, int r, PrefillWork& w, int& pair) {
   const int lane = threadIdx.x & 31;
-  if (p.batch == 1) {
-    seq = 0;
-    pair = plan.units - 1 - r;
-    return;
-  }
+  int& seq = w.seq;
+  w.parts = 1;
+  w.part = 0;
   if (plan_is_sorted(p)) {
     // lowest level with at most r pairs above it
     int lo = 0, hi = plan.top, above = 0;
@@ -202,7 +248,7 @@ __device__ __forceinline__ void find_pair(const PrefillParams& p, PrefillPlan& p
 #pragma unroll
       for (int s = 0; s < kPlanRows; ++s) {
         if (32 * s >= p.batch) break;
-        n += clamp_to(plan.base[s] + plan.pairs[s] - mid, 0, plan.pairs[s]);
+        n += clamp_to(plan.base[s] + plan.pairs[s] - mid, 0, plan.pairs[s]) * plan.parts[s];
       }
       n = __reduce_add_sync(0xffffffffu, n);
       if (n <= r)
@@ -214,14 +260,15 @@ __device__ __forceinline__ void find_pair(const PrefillParams& p, PrefillPlan& p
     seq = pair = 0;
 #pragma unroll
     for (int s = 0; s < kPlanRows; ++s) {
-      const bool here = plan.base[s] < hi && hi <= plan.base[s] + plan.pairs[s];
-      const unsigned all = __ballot_sync(0xffffffffu, here);
-      const int n = __popc(all);
+      const int here = plan.base[s] < hi && hi <= plan.base[s] + plan.pairs[s] ? plan.parts[s] : 0;
+      const int inc = warp_prefix(here);
+      const int n = __shfl_sync(0xffffffffu, inc, 31);
       if (k < n) {
-        const unsigned mine = __ballot_sync(0xffffffffu, here && __popc(all & ((1u << lane) - 1)) == k);
-        const int l = __ffs(mine) - 1;
+        const int l = __ffs(__ballot_sync(0xffffffffu, inc > k)) - 1;
         seq = 32 * s + l;
         pair = hi - __shfl_sync(0xffffffffu, plan.base[s], l) - 1;
+        w.parts = __shfl_sync(0xffffffffu, here, l);
+        w.part = k - (__shfl_sync(0xffffffffu, inc, l) - w.parts);
         break;
       }
       k -= n;
@@ -264,14 +311,31 @@ __device__ __forceinline__ void find_work(const PrefillParams& p, PrefillPlan& p
   w.seq = -1;
   w.first = w.steps[0] = w.steps[1] = w.valid[0] = w.valid[1] = 0;
   w.head = w.row0 = w.token0 = w.before = w.keys = w.open_keys = 0;
+  w.parts = 1;
+  w.part = w.slot = w.counter = 0;
   if (index >= plan.units * p.kv_heads) return;
   const int heads0 = index / (plan.units * p.head_group) * p.head_group;
   const int heads = min(p.head_group, p.kv_heads - heads0);
   const int at = index - heads0 * plan.units;
   w.head = heads0 + at % heads;
   int pair;
-  find_pair(p, plan, at / heads, w.seq, pair);
+  find_pair(p, plan, at / heads, w, pair);
   if (w.seq < 0) return;
+  if (w.parts > 1) {
+    // places in the workspace: those of the sequences before, then pair by pair
+    int slots = 0, pairs = 0;
+#pragma unroll
+    for (int s = 0; s < kPlanRows; ++s) {
+      if (32 * s + (threadIdx.x & 31) < w.seq && plan.parts[s] > 1) {
+        slots += plan.pairs[s] * plan.parts[s];
+        pairs += plan.pairs[s];
+      }
+    }
+    slots = __reduce_add_sync(0xffffffffu, slots);
+    pairs = __reduce_add_sync(0xffffffffu, pairs);
+    w.slot = (slots + pair * w.parts) * p.kv_heads + w.head * w.parts;
+    w.counter = 2 * ((pairs + pair) * p.kv_heads + w.head);
+  }
   int count;
   sequence_rows(p, w.seq, w.row0, count);
   w.keys = sequence_keys(p, w.seq, count);
@@ -284,6 +348,12 @@ __device__ __forceinline__ void find_work(const PrefillParams& p, PrefillPlan& p
     w.valid[i] = clamp_to(count - t, 0, p.tile_tokens);
     const int last = keys_of(w, t + w.valid[i] - 1);
     w.steps[i] = w.valid[i] > 0 && last > 0 ? (last + kTile - 1) / kTile : 0;
+  }
+  if (w.parts > 1) {
+    const int length = (max(w.steps[0], w.steps[1]) + w.parts - 1) / w.parts;
+    w.first = w.part * length;
+    w.steps[0] = clamp_to(w.steps[0] - w.first, 0, length);
+    w.steps[1] = clamp_to(w.steps[1] - w.first, 0, length);
   }
 }
 
@@ -315,8 +385,9 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, const uint4& v) {
 
 // Adds the non-finite values of V[key][d], key in [lo, hi), that were cleared
 // for the tile to the row `out` that sees them.
+// It is in `out`, or in column blocks of a part's O (`part`, slot_rows apart).
 __device__ __noinline__ void add_non_finite(const PrefillParams& p, int seq, int head, int row0, int dim, int lo,
-                                            int hi, __nv_bfloat16* out) {
+                                            int hi, __nv_bfloat16* out, float4* part) {
   for (int key = max(lo, 0); key < hi; ++key) {
     int64_t at;
     if (p.paged) {
@@ -330,7 +401,56 @@ __device__ __noinline__ void add_non_finite(const PrefillParams& p, int seq, int
     }
     for (int d = 0; d < dim; ++d) {
       const float x = __bfloat162float(p.v[at + d]);
-      if (!(fabsf(x) <= 3.4e38f)) out[d] = __float2bfloat16(__bfloat162float(out[d]) + x);
+      if (fabsf(x) <= 3.4e38f) continue;
+      if (part != nullptr)
+        reinterpret_cast<float*>(part + (d >> 2) * static_cast<int64_t>(p.slot_rows))[d & 3] += x;
+      else
+        out[d] = __float2bfloat16(__bfloat162float(out[d]) + x);
+    }
+  }
+}
+
+// Joins the parts of a tile's rows (128 threads, all of its warps): `slot_row`
+// is the tile's first row in a slot.  Threads share a row's columns where there
+// are fewer rows; several columns and parts are in flight per thread.
+template <int D>
+__device__ __forceinline__ void join_parts(const PrefillParams& p, int slot, int parts, int slot_row, int rows,
+                                           int tid, __nv_bfloat16* out, int64_t gap) {
+  const int shift = max(2, 32 - __clz(rows - 1));  // 2^shift rows in lanes, at least 4
+  const int r = tid & ((1 << shift) - 1), step = kTile >> shift;
+  if (r >= rows) return;
+  const int64_t slot_rows = p.slot_rows;
+  const float2* ml = p.part_ml + slot * slot_rows + slot_row + r;
+  float top = -INFINITY;
+#pragma unroll 4
+  for (int k = 0; k < parts; ++k) top = fmaxf(top, __ldcg(&ml[k * slot_rows]).x);
+  for (int c0 = tid >> shift; c0 < D / 4; c0 += 4 * step) {
+    const float4* o = p.part_o + (static_cast<int64_t>(slot) * (D / 4) + c0) * slot_rows + slot_row + r;
+    float total = 0.f, sum[16] = {};
+#pragma unroll 2
+    for (int k = 0; k < parts; ++k) {
+      const float2 v = __ldcg(&ml[k * slot_rows]);
+      if (v.y == 0.f) continue;  // saw no key: its O is not set
+      const float f = v.x == -INFINITY ? 1.f : fast_exp2((v.x - top) * p.scale_log2);
+      total += f * v.y;
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        if (c0 + m * step >= D / 4) continue;
+        const float4 a = __ldcg(&o[(k * static_cast<int64_t>(D / 4) + m * step) * slot_rows]);
+        sum[4 * m] += f * a.x;
+        sum[4 * m + 1] += f * a.y;
+        sum[4 * m + 2] += f * a.z;
+        sum[4 * m + 3] += f * a.w;
+      }
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      if (c0 + m * step >= D / 4) continue;
+      *reinterpret_cast<uint2*>(out + (r * p.group_magic >> 16) * gap + static_cast<int64_t>(r) * D +
+                                4 * (c0 + m * step)) =
+          make_uint2(pack_bf16x2(sum[4 * m] * inv, sum[4 * m + 1] * inv),
+                     pack_bf16x2(sum[4 * m + 2] * inv, sum[4 * m + 3] * inv));
     }
   }
 }
@@ -369,6 +489,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       init(sh.p_full[i], 4);
       init(sh.o_full[i], 1);
       init(sh.fix_done[i], 2);
+      init(sh.tile_sync[i], 4);
     }
     sh.abort = 0;
     sh.fix[0] = sh.fix[1] = 0;
@@ -407,6 +528,15 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       const bool pads = pad_tail < p.total || pad_head > 0;
       const int boxes = p.paged ? max(1, kTile >> p.page_shift) : 1;
       const int box_rows = kTile / boxes;
+      // Page of the box-th box of a sequence; -1 (reads as zeros) if it has none there.
+      const auto page_of = [&](const PrefillWork& w, int box) {
+        const int key = box * box_rows;
+        if (!p.paged || w.seq < 0 || key >= w.keys) return -1;
+        const int page = p.table[w.seq * p.table_stride + (key >> p.page_shift)];
+        if (static_cast<unsigned>(page) < static_cast<unsigned>(p.num_blocks)) return page;
+        atomicOr(&g_adb_error_flag, kErrCachePage);
+        return -1;
+      };
       int stage = 0, phase = 0;    // ring position of the next tile
       int loaded = 0, q_loads = 0;  // tiles, Q pairs so far
       int turn = 0;                // units handed to the other warps
@@ -444,6 +574,10 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           }
           __syncwarp();
         }
+        // page numbers of 32 / boxes tiles in the lanes, and those of the next ones on their way
+        const int ahead = 32 / boxes;
+        int pages = page_of(w, w.first * boxes + lane), next_pages = page_of(w, (w.first + ahead) * boxes + lane);
+        int tiles_left = ahead;
         for (int t = 0; t < 2 * steps; ++t) {
           if (loaded >= S) {
             wait_or_abort(&sh.kv_empty[stage], phase ^ 1, abort);
@@ -457,18 +591,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
             if ((t & 1) && tile >= w.open_keys / kTile) mbar_arrive(smem_u32(&sh.v_turn[stage]));
           }
           __syncwarp();
+          const int page = __shfl_sync(0xffffffffu, pages, (ahead - tiles_left) * boxes + lane % boxes);
           if (lane < boxes) {
             const int key = tile * kTile + lane * box_rows;
             const uint32_t dst = ring + stage * C::kTileBytes + lane * box_rows * 128;
-            int page = -1;  // outside the pool: reads as zeros
-            if (p.paged && key < w.keys) {
-              page = p.table[w.seq * p.table_stride + (key >> p.page_shift)];
-              if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_blocks)) {
-                page = -1;
-                atomicOr(&g_adb_error_flag, kErrCachePage);
-              }
-            }
             const int slot = key & ((1 << p.page_shift) - 1);
+#pragma unroll
             for (int h = 0; h < C::kHalves; ++h) {
               if (!p.paged)
                 tma_load_tile_3d(dst + h * C::kHalfBytes, map, h * 64, w.head, w.row0 + key, bar);
@@ -477,6 +605,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
               else
                 tma_load_tile_4d(dst + h * C::kHalfBytes, map, h * 64, w.head, slot, page, bar);
             }
+          }
+          if ((t & 1) && --tiles_left == 0) {
+            tiles_left = ahead;
+            pages = next_pages;
+            next_pages = page_of(w, (tile + 1 + ahead) * boxes + lane);
           }
           __syncwarp();
           ++loaded;
@@ -667,7 +800,13 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + i * kTile + lanes, o_at = tmem + 2 * kTile + i * kTile + lanes;
     const float scale = p.scale_log2;
-    int s_phase = 0, o_phase = 0;
+    int s_phase = 0, o_phase = 0, sync_phase = 0;
+    const auto sync_tile = [&] {  // (bounded, unlike a named barrier)
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.tile_sync[i]));
+      wait_or_abort(&sh.tile_sync[i], sync_phase, abort);
+      sync_phase ^= 1;
+    };
     for (int n = 0;; ++n) {
       if (!next_work(n)) break;
       const PrefillWork& w = sh.work[n & 1];
@@ -775,7 +914,39 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       const int64_t gap = static_cast<int64_t>(p.q_heads - p.group) * D;  // between the rows of two tokens
       const int rows = valid * p.group;
       const uint32_t mine = staging + i * C::kHalfBytes + (warp & 3) * 4096;
-      if ((warp & 3) * 32 < rows) {
+      if (w.parts > 1) {
+        if (rows > 0) {
+          const int r = i * p.tile_tokens * p.group + row;
+          float4* o_part = p.part_o + static_cast<int64_t>(w.slot + w.part) * (D / 4) * p.slot_rows + r;
+          if (steps > 0 && (warp & 3) * 32 < rows) {
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              float o[32];
+              tmem_ld32(o_at + c, o);
+              tmem_wait_ld();
+              if (live) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  o_part[(c / 4 + e) * static_cast<int64_t>(p.slot_rows)] =
+                      make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+              }
+            }
+            if (live && *reinterpret_cast<volatile int*>(&sh.fix[n & 1]) == n + 1)
+              add_non_finite(p, w.seq, w.head, w.row0, D, w.open_keys, w.first * kTile + sees, out, o_part);
+          }
+          if (live) p.part_ml[static_cast<int64_t>(w.slot + w.part) * p.slot_rows + r] = make_float2(top, total);
+          __threadfence();
+          sync_tile();
+          if (row == 0) {
+            const bool last = atomicAdd(&p.counters[w.counter + i], 1u) + 1 == static_cast<uint32_t>(w.parts);
+            if (last) p.counters[w.counter + i] = 0;
+            sh.last[i] = last;
+            __threadfence();
+          }
+          sync_tile();
+          if (sh.last[i]) join_parts<D>(p, w.slot, w.parts, i * p.tile_tokens * p.group, rows, row, out, gap);
+        }
+      } else if ((warp & 3) * 32 < rows) {
 #pragma unroll 1
         for (int c = 0; c < D; c += 64) {
 #pragma unroll
@@ -805,7 +976,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         }
         if (live && *reinterpret_cast<volatile int*>(&sh.fix[n & 1]) == n + 1)
           add_non_finite(p, w.seq, w.head, w.row0, D, w.open_keys, w.first * kTile + sees,
-                         out + token * gap + static_cast<int64_t>(row) * D);
+                         out + token * gap + static_cast<int64_t>(row) * D, nullptr);
       }
       tcgen05_before_sync();
       work_done(n);
