@@ -28,7 +28,7 @@ using adb_host::DeviceGuard;
 using adb_host::fail;
 using adb_host::is_aligned;
 
-constexpr int64_t kL2Bytes = 126 << 20;
+constexpr int64_t kL2Bytes = 96 << 20;  // of 126 MB, with room for Q and O
 
 int check_heads(int64_t total, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim) {
   if (total <= 0 || batch <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0)
@@ -173,11 +173,11 @@ int launch(adb::PrefillParams& p, const void* q, int64_t q_token, int64_t q_head
   p.counters = reinterpret_cast<uint32_t*>(base);
   p.part_o = reinterpret_cast<float4*>(base + ws.off_o);
   p.part_ml = reinterpret_cast<float2*>(base + ws.off_ml);
-  // KV heads worked on at a time: as many as keep the longest possible
-  // sequence's K and V within half of L2
+  // KV heads worked on at a time: even groups that keep the longest possible
+  // sequence's K and V in L2
   const int64_t keys = p.paged ? int64_t(p.max_blocks) << p.page_shift : p.total;
-  p.head_group = static_cast<int>(
-      std::max<int64_t>(1, std::min<int64_t>(p.kv_heads, kL2Bytes / 2 / std::max<int64_t>(1, keys * dim * 4))));
+const int64_t groups = std::min<int64_t>(p.kv_heads, (p.kv_heads * keys * dim * 4 + kL2Bytes - 1) / kL2Bytes);
+  p.head_group = static_cast<int>((p.kv_heads + groups - 1) / groups);
   const int64_t grid = pairs * p.kv_heads + ws.slots;
   if (grid > INT32_MAX) return fail(ADB_ERR_INVALID_ARGUMENT, "too many tiles for one call");
   if (!(flags & ADB_FLAG_HEADER_ZEROED)) {

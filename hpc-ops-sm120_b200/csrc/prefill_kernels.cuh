@@ -190,27 +190,27 @@ __device__ __forceinline__ void make_plan(const PrefillParams& p, PrefillPlan& p
     // parts of an SM's even share
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, d);
-    int share = max(kMinPart, static_cast<int>(fminf(ceilf(tiles * p.kv_heads / p.sms), 1e9f)));
-    for (bool fits = false; !fits; share *= 2) {
-      float slots = 0.f;
-#pragma unroll
-      for (int r = 0; r < kPlanRows; ++r) {
-        if (32 * r >= p.batch) break;
-        const int parts = (2 * plan.parts[r] + share) / (2 * share);
-        if (parts > 1) slots += static_cast<float>(plan.pairs[r]) * parts;
-      }
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) slots += __shfl_xor_sync(0xffffffffu, slots, d);
-      fits = slots * p.kv_heads <= p.max_slots;
-      if (!fits) continue;
+    // ... or more, until the parts of more than half a share get an SM each (if
+    // there are no more pairs than SMs) and the workspace holds the parts
+    const bool few = __reduce_add_sync(0xffffffffu, units) * p.kv_heads <= p.sms;
+    int share = max(kMinPart, static_cast<int>(fminf(ceilf(tiles * p.kv_heads / p.sms), 1e8f)));
+    for (;; share += share / 8 + 1) {
+      int slots = 0, large = 0;
       units = 0;
 #pragma unroll
       for (int r = 0; r < kPlanRows; ++r) {
         if (32 * r >= p.batch) break;
-        plan.parts[r] = max(1, (2 * plan.parts[r] + share) / (2 * share));
-        units += plan.pairs[r] * plan.parts[r];
+        const int parts = max(1, (2 * plan.parts[r] + share) / (2 * share));
+        units += plan.pairs[r] * parts;
+        if (parts > 1) slots += plan.pairs[r] * parts;
+        if (2 * plan.parts[r] > share) large += plan.pairs[r] * parts;
       }
+      slots = __reduce_add_sync(0xffffffffu, slots);
+      large = __reduce_add_sync(0xffffffffu, large);
+      if ((slots == 0) || (slots <= p.max_slots / p.kv_heads && !(few && large * p.kv_heads > p.sms))) break;
     }
+#pragma unroll
+    for (int r = 0; r < kPlanRows; ++r) plan.parts[r] = max(1, (2 * plan.parts[r] + share) / (2 * share));
   } else {
     for (int b = lane; b < p.batch; b += 32) {
       int first, count;
@@ -427,11 +427,10 @@ __device__ __forceinline__ void join_parts(const PrefillParams& p, int slot, int
   for (int c0 = tid >> shift; c0 < D / 4; c0 += 4 * step) {
     const float4* o = p.part_o + (static_cast<int64_t>(slot) * (D / 4) + c0) * slot_rows + slot_row + r;
     float total = 0.f, sum[16] = {};
-#pragma unroll 2
+#pragma unroll 4
     for (int k = 0; k < parts; ++k) {
       const float2 v = __ldcg(&ml[k * slot_rows]);
-      if (v.y == 0.f) continue;  // saw no key: its O is not set
-      const float f = v.x == -INFINITY ? 1.f : fast_exp2((v.x - top) * p.scale_log2);
+      const float f = v.x == top ? 1.f : fast_exp2((v.x - top) * p.scale_log2);
       total += f * v.y;
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
@@ -918,12 +917,14 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         if (rows > 0) {
           const int r = i * p.tile_tokens * p.group + row;
           float4* o_part = p.part_o + static_cast<int64_t>(w.slot + w.part) * (D / 4) * p.slot_rows + r;
-          if (steps > 0 && (warp & 3) * 32 < rows) {
+          if ((warp & 3) * 32 < rows) {
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
-              float o[32];
-              tmem_ld32(o_at + c, o);
-              tmem_wait_ld();
+              float o[32] = {};
+              if (steps > 0) {
+                tmem_ld32(o_at + c, o);
+                tmem_wait_ld();
+              }
               if (live) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
