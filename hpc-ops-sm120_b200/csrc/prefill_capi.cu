@@ -114,30 +114,29 @@ int prepare(int device) {
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
-// Workspace: the counters (zero between calls), then O and (maximum, total) of
-// the parts.  A part is two thirds of an SM's even share of all K/V tiles or
-// more, and the pairs of a sequence have half its tiles or more on average, so
-// that there are at most three times as many parts as SMs.
+// Workspace, of nothing but parts: O, (maximum, total), the list of what to
+// join.  A part is two thirds of an SM's even share of all K/V tiles or more,
+// and the pairs of a sequence have half its tiles or more on average, so that
+// there are at most three times as many parts as SMs.
 struct Workspace {
   int64_t slots, rows;
-  size_t header, off_o, off_ml, bytes;
+  size_t off_ml, off_joins, off_count, bytes;
 };
 
 Workspace plan_workspace(int64_t total, int64_t group, int64_t dim, int64_t sms) {
   Workspace w;
   w.slots = 3 * sms;
   w.rows = std::min<int64_t>(2 * (adb::kTile / group), total) * group;
-  w.header = static_cast<size_t>(w.slots) * sizeof(uint32_t);
-  w.off_o = align256(w.header);
-  w.off_ml = w.off_o + static_cast<size_t>(w.slots * w.rows * dim) * sizeof(float);
-  w.bytes = w.off_ml + align256(static_cast<size_t>(w.slots * w.rows) * sizeof(float2));
+  w.off_ml = align256(static_cast<size_t>(w.slots * w.rows * dim) * sizeof(float));
+  w.off_joins = w.off_ml + align256(static_cast<size_t>(w.slots * w.rows) * sizeof(float2));
+  w.off_count = w.off_joins + align256(static_cast<size_t>(w.slots / 2) * sizeof(adb::PrefillJoin));
+  w.bytes = w.off_count + 256;
   return w;
 }
 
 // `k`, the K tensor; p holds everything else.
 int launch(adb::PrefillParams& p, const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
-           int64_t k_head, int64_t dim, void* workspace, size_t workspace_bytes, unsigned flags, int device,
-           void* stream) {
+           int64_t k_head, int64_t dim, void* workspace, size_t workspace_bytes, int device, void* stream) {
   DeviceGuard guard(device);
   if (guard.error != cudaSuccess) return cuda_fail(guard.error, "cudaSetDevice");
   int sms = 0;
@@ -168,22 +167,25 @@ int launch(adb::PrefillParams& p, const void* q, int64_t q_token, int64_t q_head
     return fail(ADB_ERR_WORKSPACE, "workspace too small: %zu bytes given, %zu needed", workspace_bytes, ws.bytes);
   uint8_t* base = static_cast<uint8_t*>(workspace);
   p.sms = sms;
-  p.max_slots = static_cast<int>(ws.slots);
   p.slot_rows = static_cast<int>(ws.rows);
-  p.counters = reinterpret_cast<uint32_t*>(base);
-  p.part_o = reinterpret_cast<float4*>(base + ws.off_o);
+  p.part_o = reinterpret_cast<float*>(base);
   p.part_ml = reinterpret_cast<float2*>(base + ws.off_ml);
+  p.joins = reinterpret_cast<adb::PrefillJoin*>(base + ws.off_joins);
+  p.join_count = reinterpret_cast<int*>(base + ws.off_count);
+  // Splits need a sequence of one and a half parts.  The pairs of a prompt of n
+  // tokens have n / 256 tiles on average, so that its even share allows them
+  // only below a length.
+  const int64_t longest = p.paged ? int64_t(p.max_blocks) << p.page_shift
+                                  : std::min<int64_t>(p.total, 2 * p.tile_tokens * int64_t(sms) * 4 / (3 * p.kv_heads));
+  const bool splits = longest > (3 * adb::kMinPart / 2 - 1) * adb::kTile;
+  p.max_slots = splits ? static_cast<int>(ws.slots) : 0;
   // KV heads worked on at a time: even groups that keep the longest possible
   // sequence's K and V in L2
   const int64_t keys = p.paged ? int64_t(p.max_blocks) << p.page_shift : p.total;
 const int64_t groups = std::min<int64_t>(p.kv_heads, (p.kv_heads * keys * dim * 4 + kL2Bytes - 1) / kL2Bytes);
   p.head_group = static_cast<int>((p.kv_heads + groups - 1) / groups);
-  const int64_t grid = pairs * p.kv_heads + ws.slots;
+  const int64_t grid = pairs * p.kv_heads + p.max_slots;
   if (grid > INT32_MAX) return fail(ADB_ERR_INVALID_ARGUMENT, "too many tiles for one call");
-  if (!(flags & ADB_FLAG_HEADER_ZEROED)) {
-    const cudaError_t me = cudaMemsetAsync(workspace, 0, ws.header, static_cast<cudaStream_t>(stream));
-    if (me != cudaSuccess) return cuda_fail(me, "workspace header memset");
-  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(adb::kPrefillThreads);
@@ -194,9 +196,17 @@ const int64_t groups = std::min<int64_t>(p.kv_heads, (p.kv_heads * keys * dim * 
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = dim == 128 ? cudaLaunchKernelEx(&cfg, adb::prefill_kernel<128>, q_map, k_map, v_map, p)
-                                   : cudaLaunchKernelEx(&cfg, adb::prefill_kernel<64>, q_map, k_map, v_map, p);
+  cudaError_t e = dim == 128 ? cudaLaunchKernelEx(&cfg, adb::prefill_kernel<128>, q_map, k_map, v_map, p)
+                             : cudaLaunchKernelEx(&cfg, adb::prefill_kernel<64>, q_map, k_map, v_map, p);
   if (e != cudaSuccess) return cuda_fail(e, "prefill kernel launch");
+  adb_host::count_launch();
+  if (!splits) return ADB_OK;
+  const int64_t join_rows = ws.slots / 2 * ws.rows;
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(4 * sms, (join_rows + 7) / 8)));
+  cfg.blockDim = dim3(adb::kJoinThreads);
+  cfg.dynamicSmemBytes = 0;
+  e = cudaLaunchKernelEx(&cfg, dim == 128 ? adb::prefill_join_kernel<128> : adb::prefill_join_kernel<64>, p);
+  if (e != cudaSuccess) return cuda_fail(e, "prefill join kernel launch");
   adb_host::count_launch();
   return ADB_OK;
 }
@@ -215,7 +225,7 @@ int adb_prefill_workspace_size(int64_t total, int64_t batch, int64_t q_heads, in
   if (status != ADB_OK) return status;
   const Workspace w = plan_workspace(total, q_heads / kv_heads, head_dim, sms);
   *bytes = w.bytes;
-  if (header_bytes != nullptr) *header_bytes = w.header;
+  if (header_bytes != nullptr) *header_bytes = 0;
   return ADB_OK;
 }
 
@@ -243,7 +253,7 @@ int adb_prefill(const void* q, int64_t q_token_stride, int64_t q_head_stride, co
   p.kv_heads = static_cast<int>(kv_heads);
   p.group = static_cast<int>(q_heads / kv_heads);
   return launch(p, q, q_token_stride, q_head_stride, k, k_token_stride, k_head_stride, head_dim, workspace,
-                workspace_bytes, flags, device, stream);
+                workspace_bytes, device, stream);
 }
 
 int adb_prefill_paged(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
@@ -290,8 +300,8 @@ int adb_prefill_paged(const void* q, int64_t q_token_stride, int64_t q_head_stri
   p.max_blocks = static_cast<int>(max_blocks_per_seq);
   p.num_blocks = static_cast<int>(num_blocks);
   while ((int64_t(1) << p.page_shift) < page_size) ++p.page_shift;
-  return launch(p, q, q_token_stride, q_head_stride, k_cache, 0, 0, head_dim, workspace, workspace_bytes, flags,
-                device, stream);
+  return launch(p, q, q_token_stride, q_head_stride, k_cache, 0, 0, head_dim, workspace, workspace_bytes, device,
+                stream);
 }
 
 }  // extern "C"

@@ -20,9 +20,10 @@
 //
 // Splits.  Where a sequence's K/V tiles are one and a half times an SM's even
 // share of all tiles or more (few rows over a long cache), its pairs are cut
-// into parts of about that share.  A part leaves its unnormalised O and (maximum, total) in the
-// workspace; the part of a tile that finishes last joins them, in the order of
-// the parts, so that the result does not depend on which one that is.
+// into parts of about that share.  A part leaves its unnormalised O and
+// (maximum, total) in the workspace, and a second kernel joins them, a warp per
+// row.  (Joined in the CTA of the part that finishes last, 256 rows of 16 parts
+// took 45 us.)
 //
 // Pipeline of a CTA (384 threads):
 //   warps 0-3, 4-7   softmax of tile 0, 1: one thread per row
@@ -76,9 +77,18 @@ struct PrefillParams {
   int sms;
   int max_slots;           // parts that the workspace holds (0: no splits)
   int slot_rows;           // rows of a part: group times the tokens of a pair, or of all sequences
-  uint32_t* counters;      // [max_slots] finished parts per tile of a pair, zero between calls
-  float4* part_o;          // [max_slots][D / 4][slot_rows]
+  float* part_o;           // [max_slots][slot_rows][D]
   float2* part_ml;         // [max_slots][slot_rows] maximum (of q . k), total
+  struct PrefillJoin* joins;  // [max_slots / 2] pairs cut into parts
+  int* join_count;
+};
+
+// A pair of tiles whose parts are to be joined.
+struct PrefillJoin {
+  int row;     // of its first token in out
+  int rows;    // of both tiles
+  int head;    // KV head
+  int slot, parts;
 };
 
 template <int D>
@@ -104,7 +114,7 @@ struct PrefillWork {
   int open_keys;     // keys from here on are hidden from some row of the tiles
   int parts, part;   // of the pair's K/V tiles
   int slot;          // of the pair's part 0 in the workspace
-  int counter;       // of tile 0
+  int join;          // its place among the pairs cut into parts
   int pad_head, pad_tail;  // rows before the first / from the end of the last sequence
 };
 
@@ -119,10 +129,8 @@ struct PrefillShared {
   uint64_t v_turn[PrefillCfg<D>::kStages];   // a border tile of V is on its way
   uint64_t v_clean[PrefillCfg<D>::kStages];  // and cleared
   uint64_t fix_done[2];
-  uint64_t tile_sync[2];  // the four warps of a tile
   uint32_t tmem;
   int abort;
-  int last[2];       // this CTA's part of tile i finished last
   int fix[2];        // number of the unit of which a non-finite value of V was cleared
   PrefillWork work[2];
 };
@@ -146,6 +154,7 @@ struct PrefillPlan {
   int pairs[kPlanRows], base[kPlanRows];
   int parts[kPlanRows];            // of each of a sequence's pairs
   int units;                       // parts of all pairs of all sequences
+  int joins;                       // pairs cut into parts
   int top;                         // highest level
   int scan_base, scan_before;      // where the walk stands
 };
@@ -162,7 +171,7 @@ __device__ __forceinline__ int pairs_of(const PrefillParams& p, int count) {
 
 __device__ __forceinline__ void make_plan(const PrefillParams& p, PrefillPlan& plan) {
   const int lane = threadIdx.x & 31;
-  plan.scan_base = plan.scan_before = 0;
+  plan.scan_base = plan.scan_before = plan.joins = 0;
   int units = 0, top = 0;
   float tiles = 0.f;  // K/V tiles of all pairs
 #pragma unroll
@@ -194,7 +203,7 @@ __device__ __forceinline__ void make_plan(const PrefillParams& p, PrefillPlan& p
     // there are no more pairs than SMs) and the workspace holds the parts
     const bool few = __reduce_add_sync(0xffffffffu, units) * p.kv_heads <= p.sms;
     int share = max(kMinPart, static_cast<int>(fminf(ceilf(tiles * p.kv_heads / p.sms), 1e8f)));
-    for (;; share += share / 8 + 1) {
+    for (; p.max_slots > 0; share += share / 8 + 1) {
       int slots = 0, large = 0;
       units = 0;
 #pragma unroll
@@ -207,10 +216,17 @@ __device__ __forceinline__ void make_plan(const PrefillParams& p, PrefillPlan& p
       }
       slots = __reduce_add_sync(0xffffffffu, slots);
       large = __reduce_add_sync(0xffffffffu, large);
-      if ((slots == 0) || (slots <= p.max_slots / p.kv_heads && !(few && large * p.kv_heads > p.sms))) break;
+      if (slots == 0 || (slots <= p.max_slots / p.kv_heads && !(few && large * p.kv_heads > p.sms))) break;
     }
 #pragma unroll
-    for (int r = 0; r < kPlanRows; ++r) plan.parts[r] = max(1, (2 * plan.parts[r] + share) / (2 * share));
+    for (int r = 0; r < kPlanRows; ++r) {
+      plan.parts[r] = p.max_slots > 0 ? max(1, (2 * plan.parts[r] + share) / (2 * share)) : 1;
+      if (plan.parts[r] > 1) {
+        plan.joins += plan.pairs[r];
+        plan.base[r] /= plan.parts[r];  // the order goes by a part's length
+        // (the highest level stays an upper bound)
+      }
+    }
   } else {
     for (int b = lane; b < p.batch; b += 32) {
       int first, count;
@@ -220,6 +236,7 @@ __device__ __forceinline__ void make_plan(const PrefillParams& p, PrefillPlan& p
   }
   plan.units = __reduce_add_sync(0xffffffffu, units);
   plan.top = __reduce_max_sync(0xffffffffu, top);
+  plan.joins = __reduce_add_sync(0xffffffffu, plan.joins);
 }
 
 // Inclusive prefix of v over the warp.
@@ -312,7 +329,7 @@ __device__ __forceinline__ void find_work(const PrefillParams& p, PrefillPlan& p
   w.first = w.steps[0] = w.steps[1] = w.valid[0] = w.valid[1] = 0;
   w.head = w.row0 = w.token0 = w.before = w.keys = w.open_keys = 0;
   w.parts = 1;
-  w.part = w.slot = w.counter = 0;
+  w.part = w.slot = w.join = 0;
   if (index >= plan.units * p.kv_heads) return;
   const int heads0 = index / (plan.units * p.head_group) * p.head_group;
   const int heads = min(p.head_group, p.kv_heads - heads0);
@@ -334,7 +351,7 @@ __device__ __forceinline__ void find_work(const PrefillParams& p, PrefillPlan& p
     slots = __reduce_add_sync(0xffffffffu, slots);
     pairs = __reduce_add_sync(0xffffffffu, pairs);
     w.slot = (slots + pair * w.parts) * p.kv_heads + w.head * w.parts;
-    w.counter = 2 * ((pairs + pair) * p.kv_heads + w.head);
+    w.join = (pairs + pair) * p.kv_heads + w.head;
   }
   int count;
   sequence_rows(p, w.seq, w.row0, count);
@@ -385,9 +402,9 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, const uint4& v) {
 
 // Adds the non-finite values of V[key][d], key in [lo, hi), that were cleared
 // for the tile to the row `out` that sees them.
-// It is in `out`, or in column blocks of a part's O (`part`, slot_rows apart).
+// It is in `out`, or in a part's O (`part`).
 __device__ __noinline__ void add_non_finite(const PrefillParams& p, int seq, int head, int row0, int dim, int lo,
-                                            int hi, __nv_bfloat16* out, float4* part) {
+                                            int hi, __nv_bfloat16* out, float* part) {
   for (int key = max(lo, 0); key < hi; ++key) {
     int64_t at;
     if (p.paged) {
@@ -403,53 +420,9 @@ __device__ __noinline__ void add_non_finite(const PrefillParams& p, int seq, int
       const float x = __bfloat162float(p.v[at + d]);
       if (fabsf(x) <= 3.4e38f) continue;
       if (part != nullptr)
-        reinterpret_cast<float*>(part + (d >> 2) * static_cast<int64_t>(p.slot_rows))[d & 3] += x;
+        part[d] += x;
       else
         out[d] = __float2bfloat16(__bfloat162float(out[d]) + x);
-    }
-  }
-}
-
-// Joins the parts of a tile's rows (128 threads, all of its warps): `slot_row`
-// is the tile's first row in a slot.  Threads share a row's columns where there
-// are fewer rows; several columns and parts are in flight per thread.
-template <int D>
-__device__ __forceinline__ void join_parts(const PrefillParams& p, int slot, int parts, int slot_row, int rows,
-                                           int tid, __nv_bfloat16* out, int64_t gap) {
-  const int shift = max(2, 32 - __clz(rows - 1));  // 2^shift rows in lanes, at least 4
-  const int r = tid & ((1 << shift) - 1), step = kTile >> shift;
-  if (r >= rows) return;
-  const int64_t slot_rows = p.slot_rows;
-  const float2* ml = p.part_ml + slot * slot_rows + slot_row + r;
-  float top = -INFINITY;
-#pragma unroll 4
-  for (int k = 0; k < parts; ++k) top = fmaxf(top, __ldcg(&ml[k * slot_rows]).x);
-  for (int c0 = tid >> shift; c0 < D / 4; c0 += 4 * step) {
-    const float4* o = p.part_o + (static_cast<int64_t>(slot) * (D / 4) + c0) * slot_rows + slot_row + r;
-    float total = 0.f, sum[16] = {};
-#pragma unroll 4
-    for (int k = 0; k < parts; ++k) {
-      const float2 v = __ldcg(&ml[k * slot_rows]);
-      const float f = v.x == top ? 1.f : fast_exp2((v.x - top) * p.scale_log2);
-      total += f * v.y;
-#pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        if (c0 + m * step >= D / 4) continue;
-        const float4 a = __ldcg(&o[(k * static_cast<int64_t>(D / 4) + m * step) * slot_rows]);
-        sum[4 * m] += f * a.x;
-        sum[4 * m + 1] += f * a.y;
-        sum[4 * m + 2] += f * a.z;
-        sum[4 * m + 3] += f * a.w;
-      }
-    }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-#pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      if (c0 + m * step >= D / 4) continue;
-      *reinterpret_cast<uint2*>(out + (r * p.group_magic >> 16) * gap + static_cast<int64_t>(r) * D +
-                                4 * (c0 + m * step)) =
-          make_uint2(pack_bf16x2(sum[4 * m] * inv, sum[4 * m + 1] * inv),
-                     pack_bf16x2(sum[4 * m + 2] * inv, sum[4 * m + 3] * inv));
     }
   }
 }
@@ -488,7 +461,6 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       init(sh.p_full[i], 4);
       init(sh.o_full[i], 1);
       init(sh.fix_done[i], 2);
-      init(sh.tile_sync[i], 4);
     }
     sh.abort = 0;
     sh.fix[0] = sh.fix[1] = 0;
@@ -524,6 +496,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       const int pad_tail = clamp_to(p.cu[p.batch], 0, p.total), pad_head = clamp_to(p.cu[0], 0, p.total);
       PrefillPlan plan;
       make_plan(p, plan);
+      if (p.max_slots > 0 && blockIdx.x == 0 && lane == 0) *p.join_count = plan.joins * p.kv_heads;
       const bool pads = pad_tail < p.total || pad_head > 0;
       const int boxes = p.paged ? max(1, kTile >> p.page_shift) : 1;
       const int box_rows = kTile / boxes;
@@ -799,13 +772,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + i * kTile + lanes, o_at = tmem + 2 * kTile + i * kTile + lanes;
     const float scale = p.scale_log2;
-    int s_phase = 0, o_phase = 0, sync_phase = 0;
-    const auto sync_tile = [&] {  // (bounded, unlike a named barrier)
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh.tile_sync[i]));
-      wait_or_abort(&sh.tile_sync[i], sync_phase, abort);
-      sync_phase ^= 1;
-    };
+    int s_phase = 0, o_phase = 0;
     for (int n = 0;; ++n) {
       if (!next_work(n)) break;
       const PrefillWork& w = sh.work[n & 1];
@@ -914,39 +881,38 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       const int rows = valid * p.group;
       const uint32_t mine = staging + i * C::kHalfBytes + (warp & 3) * 4096;
       if (w.parts > 1) {
-        if (rows > 0) {
-          const int r = i * p.tile_tokens * p.group + row;
-          float4* o_part = p.part_o + static_cast<int64_t>(w.slot + w.part) * (D / 4) * p.slot_rows + r;
-          if ((warp & 3) * 32 < rows) {
+        const int64_t first_row = static_cast<int64_t>(w.slot + w.part) * p.slot_rows + i * p.tile_tokens * p.group;
+        if ((warp & 3) * 32 < rows) {
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              float o[32] = {};
-              if (steps > 0) {
-                tmem_ld32(o_at + c, o);
-                tmem_wait_ld();
-              }
-              if (live) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                  o_part[(c / 4 + e) * static_cast<int64_t>(p.slot_rows)] =
-                      make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-              }
+          for (int c = 0; c < D; c += 32) {
+            float o[32] = {};
+            if (steps > 0) {
+              tmem_ld32(o_at + c, o);
+              tmem_wait_ld();
             }
-            if (live && *reinterpret_cast<volatile int*>(&sh.fix[n & 1]) == n + 1)
-              add_non_finite(p, w.seq, w.head, w.row0, D, w.open_keys, w.first * kTile + sees, out, o_part);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              st_shared_v4(mine + lane * 128 + (e ^ (lane & 7)) * 16,
+                           make_uint4(__float_as_uint(o[4 * e]), __float_as_uint(o[4 * e + 1]),
+                                      __float_as_uint(o[4 * e + 2]), __float_as_uint(o[4 * e + 3])));
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int l = 4 * k + (lane >> 3), x = lane & 7, r = (warp & 3) * 32 + l;
+              const uint4 v = ld_shared_v4(mine + l * 128 + (x ^ (l & 7)) * 16);
+              if (r < rows) *reinterpret_cast<uint4*>(p.part_o + (first_row + r) * D + c + x * 4) = v;
+            }
+            __syncwarp();
           }
-          if (live) p.part_ml[static_cast<int64_t>(w.slot + w.part) * p.slot_rows + r] = make_float2(top, total);
-          __threadfence();
-          sync_tile();
-          if (row == 0) {
-            const bool last = atomicAdd(&p.counters[w.counter + i], 1u) + 1 == static_cast<uint32_t>(w.parts);
-            if (last) p.counters[w.counter + i] = 0;
-            sh.last[i] = last;
-            __threadfence();
+          if (live) {
+            p.part_ml[first_row + row] = make_float2(top, total);
+            if (*reinterpret_cast<volatile int*>(&sh.fix[n & 1]) == n + 1)
+              add_non_finite(p, w.seq, w.head, w.row0, D, w.open_keys, w.first * kTile + sees, out,
+                             p.part_o + (first_row + row) * D);
           }
-          sync_tile();
-          if (sh.last[i]) join_parts<D>(p, w.slot, w.parts, i * p.tile_tokens * p.group, rows, row, out, gap);
         }
+        if (tid == 0 && w.part == 0)
+          p.joins[w.join] = {w.row0 + w.token0, (w.valid[0] + w.valid[1]) * p.group, w.head, w.slot, w.parts};
       } else if ((warp & 3) * 32 < rows) {
 #pragma unroll 1
         for (int c = 0; c < D; c += 64) {
@@ -990,6 +956,70 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     tcgen05_after_sync();
     tmem_dealloc(tmem, 512);
   }
+}
+
+// Joins the parts, a warp per row:
+//   M = max m, o = sum e^(m - M) O / sum e^(m - M) l.
+constexpr int kJoinThreads = 256;
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) prefill_join_kernel(const __grid_constant__ PrefillParams p) {
+  constexpr int kLanes = D / 4;         // of a row of O, 16 bytes each
+  constexpr int kAtOnce = 32 / kLanes;  // parts that a warp reads at a time
+  const int lane = threadIdx.x & 31;
+  const int warps = gridDim.x * (kJoinThreads / 32);
+  griddep_wait();
+  const int64_t rows = static_cast<int64_t>(__ldcg(p.join_count)) * p.slot_rows;
+  for (int64_t x = blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5); x < rows; x += warps) {
+    const int* words = reinterpret_cast<const int*>(p.joins + x / p.slot_rows);
+    const PrefillJoin j = {__ldcg(words), __ldcg(words + 1), __ldcg(words + 2), __ldcg(words + 3), __ldcg(words + 4)};
+    const int r = static_cast<int>(x % p.slot_rows);
+    if (r >= j.rows) continue;
+    const float2* ml = p.part_ml + static_cast<int64_t>(j.slot) * p.slot_rows + r;
+    const float* o = p.part_o + (static_cast<int64_t>(j.slot) * p.slot_rows + r) * D + (lane % kLanes) * 4;
+    float top = -INFINITY;
+    for (int k = lane; k < j.parts; k += 32) top = fmaxf(top, __ldcg(&ml[static_cast<int64_t>(k) * p.slot_rows]).x);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    float total = 0.f;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = 0; k0 < j.parts; k0 += 32) {
+      float f = 0.f;
+      if (k0 + lane < j.parts) {
+        const float2 v = __ldcg(&ml[static_cast<int64_t>(k0 + lane) * p.slot_rows]);
+        f = v.x == top ? 1.f : fast_exp2((v.x - top) * p.scale_log2);
+        total += f * v.y;
+      }
+      const int n = min(32, j.parts - k0);
+#pragma unroll 4
+      for (int k = 0; k < n; k += kAtOnce) {
+        const int mine = k + lane / kLanes;
+        const float g = __shfl_sync(0xffffffffu, f, mine & 31);
+        if (mine < n) {
+          const float4 a = __ldcg(reinterpret_cast<const float4*>(o + static_cast<int64_t>(k0 + mine) * p.slot_rows * D));
+          sum.x += g * a.x;
+          sum.y += g * a.y;
+          sum.z += g * a.z;
+          sum.w += g * a.w;
+        }
+      }
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+#pragma unroll
+    for (int d = 16; d >= kLanes; d >>= 1) {
+      sum.x += __shfl_xor_sync(0xffffffffu, sum.x, d);
+      sum.y += __shfl_xor_sync(0xffffffffu, sum.y, d);
+      sum.z += __shfl_xor_sync(0xffffffffu, sum.z, d);
+      sum.w += __shfl_xor_sync(0xffffffffu, sum.w, d);
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    if (lane < kLanes) {
+      const int64_t row = static_cast<int64_t>(j.row + r / p.group) * p.q_heads + j.head * p.group + r % p.group;
+      *reinterpret_cast<uint2*>(p.out + row * D + lane * 4) =
+          make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
+    }
+  }
+  griddep_launch_dependents();
 }
 
 }  // namespace adb
