@@ -53,8 +53,8 @@ int encode(CUtensorMap* map, const void* base, int rank, const int64_t* dims, co
   PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   const int rc = adb_host::get_encoder(&fn);
   if (rc != ADB_OK) return rc;
-  cuuint64_t d[4], s[3];
-  cuuint32_t b[4], one[4] = {1u, 1u, 1u, 1u};
+  cuuint64_t d[5], s[4];
+  cuuint32_t b[5], one[5] = {1u, 1u, 1u, 1u, 1u};
   for (int i = 0; i < rank; ++i) {
     d[i] = static_cast<cuuint64_t>(dims[i]);
     b[i] = static_cast<cuuint32_t>(box[i]);
@@ -75,33 +75,35 @@ int encode_packed(CUtensorMap* map, const void* base, int64_t tokens, int64_t he
   return encode(map, base, 3, dims, strides, box);
 }
 
-int encode_pages(CUtensorMap* map, const void* base, const adb::PrefillParams& p, int64_t dim) {
-  const int64_t page = int64_t(1) << p.page_shift;
+// Pages of either layout as [blocks][heads][64-column blocks][tokens][64].
+int encode_pages(CUtensorMap* map, const void* base, const adb::PrefillParams& p, int64_t dim, bool pair) {
+  const int64_t page = int64_t(1) << p.page_shift, heads = p.kv_heads;
   const int rows = static_cast<int>(page < adb::kTile ? page : adb::kTile);
-  if (p.paged == 1) {
-    const int64_t dims[4] = {dim, page, p.kv_heads, p.num_blocks}, strides[4] = {1, dim, page * dim, p.kv_heads * page * dim};
-    const int box[4] = {64, rows, 1, 1};
-    return encode(map, base, 4, dims, strides, box);
-  }
-  const int64_t dims[4] = {dim, p.kv_heads, page, p.num_blocks}, strides[4] = {1, dim, p.kv_heads * dim, p.kv_heads * page * dim};
-  const int box[4] = {64, 1, rows, 1};
-  return encode(map, base, 4, dims, strides, box);
+  const bool hnd = p.paged == 1;
+  const int64_t dims[5] = {64, page, dim / 64, heads, p.num_blocks};
+  const int64_t strides[5] = {1, hnd ? dim : heads * dim, 64, hnd ? page * dim : dim, heads * page * dim};
+  const int box[5] = {64, rows, pair ? 2 : 1, 1, 1};
+  return encode(map, base, 5, dims, strides, box);
 }
 
-// The kernel's shared-memory limit is set once per device.
+struct Kernel {
+  void (*run)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const adb::PrefillParams);
+  int smem;
+};
+const Kernel kKernels[] = {{adb::prefill_kernel<64, false>, adb::PrefillCfg<64>::kSmemBytes},
+                           {adb::prefill_kernel<128, false>, adb::PrefillCfg<128>::kSmemBytes},
+                           {adb::prefill_kernel<128, true>, adb::PrefillCfg<128>::kSmemBytes}};
+
+// Once per device: the kernels' shared-memory limit, and that they were
+// compiled to the registers that the split between their warps counts on.
 int prepare(int device) {
   static std::atomic<uint64_t> done{0};
   const uint64_t bit = uint64_t(1) << device;
   if (done.load(std::memory_order_acquire) & bit) return ADB_OK;
-  cudaError_t e = cudaFuncSetAttribute(&adb::prefill_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       adb::PrefillCfg<128>::kSmemBytes);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(&adb::prefill_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             adb::PrefillCfg<64>::kSmemBytes);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(max dynamic smem)");
-  // The warps' register split counts on what the block is launched with.
-  for (const void* fn : {reinterpret_cast<const void*>(&adb::prefill_kernel<128>),
-                         reinterpret_cast<const void*>(&adb::prefill_kernel<64>)}) {
+  for (const Kernel& k : kKernels) {
+    const void* fn = reinterpret_cast<const void*>(k.run);
+    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(max dynamic smem)");
     cudaFuncAttributes a;
     e = cudaFuncGetAttributes(&a, fn);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncGetAttributes");
@@ -146,12 +148,16 @@ int launch(adb::PrefillParams& p, const void* q, int64_t q_token, int64_t q_head
   p.scale_log2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(dim)));
   p.tile_tokens = adb::kTile / p.group;
   p.group_magic = (65536 + p.group - 1) / p.group;
+  // one box of both 64-column blocks where a page is too small to pay for two
+  // (one token over 131072, pages of 8 / 16 / 64 tokens: 180 / 119 / 105 us with
+  // two, 118 / 110 us with one)
+  const bool pair = p.paged && dim == 128 && p.page_shift <= 4;
   CUtensorMap q_map, k_map, v_map;
   rc = encode_packed(&q_map, q, p.total, p.q_heads, dim, q_token, q_head, p.group, p.tile_tokens);
   if (rc != ADB_OK) return rc;
   if (p.paged) {
-    rc = encode_pages(&k_map, k, p, dim);
-    if (rc == ADB_OK) rc = encode_pages(&v_map, p.v, p, dim);
+    rc = encode_pages(&k_map, k, p, dim, pair);
+    if (rc == ADB_OK) rc = encode_pages(&v_map, p.v, p, dim, pair);
   } else {
     rc = encode_packed(&k_map, k, p.total, p.kv_heads, dim, k_token, k_head, 1, adb::kTile);
     if (rc == ADB_OK) rc = encode_packed(&v_map, p.v, p.total, p.kv_heads, dim, p.v_token, p.v_head, 1, adb::kTile);
@@ -189,15 +195,15 @@ const int64_t groups = std::min<int64_t>(p.kv_heads, (p.kv_heads * keys * dim * 
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(adb::kPrefillThreads);
-  cfg.dynamicSmemBytes = dim == 128 ? adb::PrefillCfg<128>::kSmemBytes : adb::PrefillCfg<64>::kSmemBytes;
+  const Kernel& kernel = kKernels[dim == 64 ? 0 : pair ? 2 : 1];
+  cfg.dynamicSmemBytes = static_cast<size_t>(kernel.smem);
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = dim == 128 ? cudaLaunchKernelEx(&cfg, adb::prefill_kernel<128>, q_map, k_map, v_map, p)
-                             : cudaLaunchKernelEx(&cfg, adb::prefill_kernel<64>, q_map, k_map, v_map, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel.run, q_map, k_map, v_map, p);
   if (e != cudaSuccess) return cuda_fail(e, "prefill kernel launch");
   adb_host::count_launch();
   if (!splits) return ADB_OK;

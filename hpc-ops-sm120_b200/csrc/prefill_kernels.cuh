@@ -25,6 +25,12 @@
 // row.  (Joined in the CTA of the part that finishes last, 256 rows of 16 parts
 // took 45 us.)
 //
+// Small pages.  The TMA unit takes about 70 cycles per box, whatever it holds,
+// so pages of 8 and 16 tokens come as one box of both 64-column blocks (D 128).
+// A page's rows of a block then lie behind its rows of the other, and the rows
+// 8 r .. 8 r + 7 of all pages are one operand (pages are its stride): the keys
+// of a tile are taken in the order r, page, row (tile_key), in S, P and V alike.
+//
 // Pipeline of a CTA (384 threads):
 //   warps 0-3, 4-7   softmax of tile 0, 1: one thread per row
 //   warp 8           finds the units; TMA loads: Q, then K_0 V_0 K_1 V_1 ...
@@ -117,6 +123,9 @@ struct PrefillWork {
   int join;          // its place among the pairs cut into parts
   int pad_head, pad_tail;  // rows before the first / from the end of the last sequence
 };
+
+// Key of a tile in column c of S, for pages of 16 tokens that come as one box.
+__host__ __device__ constexpr int tile_key16(int c) { return ((c & 63) >> 3) * 16 + (c >> 6) * 8 + (c & 7); }
 
 template <int D>
 struct PrefillShared {
@@ -427,7 +436,8 @@ __device__ __noinline__ void add_non_finite(const PrefillParams& p, int seq, int
   }
 }
 
-template <int D>
+// kPair: pages come as one box of both column blocks (small pages, D 128).
+template <int D, bool kPair>
 __global__ void __launch_bounds__(kPrefillThreads, 1)
     prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                    const __grid_constant__ CUtensorMap v_map, const __grid_constant__ PrefillParams p) {
@@ -566,16 +576,19 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           const int page = __shfl_sync(0xffffffffu, pages, (ahead - tiles_left) * boxes + lane % boxes);
           if (lane < boxes) {
             const int key = tile * kTile + lane * box_rows;
-            const uint32_t dst = ring + stage * C::kTileBytes + lane * box_rows * 128;
+            const uint32_t dst = ring + stage * C::kTileBytes;
             const int slot = key & ((1 << p.page_shift) - 1);
+            if (kPair) {
+              tma_load_tile_5d(dst + lane * box_rows * C::kHalves * 128, map, 0, slot, 0, w.head, page, bar);
+            } else {
 #pragma unroll
-            for (int h = 0; h < C::kHalves; ++h) {
-              if (!p.paged)
-                tma_load_tile_3d(dst + h * C::kHalfBytes, map, h * 64, w.head, w.row0 + key, bar);
-              else if (p.paged == 1)
-                tma_load_tile_4d(dst + h * C::kHalfBytes, map, h * 64, slot, w.head, page, bar);
-              else
-                tma_load_tile_4d(dst + h * C::kHalfBytes, map, h * 64, w.head, slot, page, bar);
+              for (int h = 0; h < C::kHalves; ++h) {
+                const uint32_t at = dst + h * C::kHalfBytes + lane * box_rows * 128;
+                if (p.paged)
+                  tma_load_tile_5d(at, map, 0, slot, h, w.head, page, bar);
+                else
+                  tma_load_tile_3d(at, map, h * 64, w.head, w.row0 + key, bar);
+              }
             }
           }
           if ((t & 1) && --tiles_left == 0) {
@@ -612,29 +625,44 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       // one lane's branch an MMA took 65 cycles to issue, and the issue was
       // what bounded the kernel (567 us for 8192 tokens, 32/8 heads, D 128).
       constexpr uint64_t k_major = smem_desc_base(16, 1024);
-      constexpr uint64_t v_major = smem_desc_base(C::kHalfBytes, 1024);
+      const bool pair16 = kPair && p.page_shift == 4;
+      const uint32_t page_bytes = 256u << p.page_shift;  // of both column blocks
+      const uint64_t k_ring = kPair ? smem_desc_base(16, page_bytes) : k_major;
+      const uint64_t v_ring = kPair ? smem_desc_base(page_bytes / 2, page_bytes) : smem_desc_base(C::kHalfBytes, 1024);
+      const uint32_t k_half = (kPair ? page_bytes / 2 : C::kHalfBytes) >> 4;
       constexpr uint32_t qk_idesc = mma_idesc(kTile, kTile, false);
+      constexpr uint32_t qk16_idesc = mma_idesc(kTile, kTile / 2, false);
       constexpr uint32_t pv_idesc = mma_idesc(kTile, D, true);
       const auto qk = [&](int i, int stage) {
         const uint64_t a = smem_desc(k_major, tiles + i * C::kTileBytes);
-        const uint64_t b = smem_desc(k_major, ring + stage * C::kTileBytes);
+        const uint64_t b = smem_desc(k_ring, ring + stage * C::kTileBytes);
         if (elect_one()) {
+          if (pair16) {
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t at = ((k >> 2) * C::kHalfBytes + (k & 3) * 32) >> 4;
-            mma_ss(tmem + i * kTile, a + at, b + at, qk_idesc, k > 0);
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int k = 0; k < D / 16; ++k)
+                mma_ss(tmem + i * kTile + r * (kTile / 2), a + ((k >> 2) * (C::kHalfBytes >> 4) + (k & 3) * 2),
+                       b + (r * (1024 >> 4) + (k >> 2) * k_half + (k & 3) * 2), qk16_idesc, k > 0);
+          } else {
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+              mma_ss(tmem + i * kTile, a + ((k >> 2) * (C::kHalfBytes >> 4) + (k & 3) * 2),
+                     b + ((k >> 2) * k_half + (k & 3) * 2), qk_idesc, k > 0);
           }
           mma_commit(smem_u32(&sh.s_full[i]));
         }
         __syncwarp();
       };
       const auto pv = [&](int i, int stage, int first, int last, bool accumulate) {
-        const uint64_t v = smem_desc(v_major, ring + stage * C::kTileBytes);
+        const uint64_t v = smem_desc(v_ring, ring + stage * C::kTileBytes);
+        // from one 16 keys to the next: two pages of 8 rows, or half of all pages' rows and then the other
+        const uint32_t step = (kPair ? 2 * page_bytes : 2048) >> 4;
         if (elect_one()) {
 #pragma unroll
           for (int k = first; k < last; ++k)
-            mma_ts(tmem + 2 * kTile + i * kTile, tmem + i * kTile + k * 8, v + k * (2048 >> 4), pv_idesc,
-                   accumulate || k > 0);
+            mma_ts(tmem + 2 * kTile + i * kTile, tmem + i * kTile + k * 8,
+                   v + (pair16 ? (k & 3) * step + (k >> 2) * (1024 >> 4) : k * step), pv_idesc, accumulate || k > 0);
         }
         __syncwarp();
       };
@@ -720,7 +748,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
             const int first = 8 * max(open_keys - tile * kTile, 0);           // first vector that some row may not see
             const int behind = 8 * clamp_to(keys - tile * kTile, 0, kTile);  // first vector behind the sequence
             for (int h = 0; h < C::kHalves; ++h) {
-              const uint32_t base = ring + stage * C::kTileBytes + h * C::kHalfBytes;
+              const uint32_t tile_at = ring + stage * C::kTileBytes;
+              const auto vector_at = [&](int x) {  // x-th vector of the column block, 8 per key
+                if (!kPair) return tile_at + h * C::kHalfBytes + x * 16;
+                const int shift = p.page_shift + 3;
+                return tile_at + (((x >> shift) * C::kHalves + h) << (shift + 4)) + (x & ((1 << shift) - 1)) * 16;
+              };
               for (int x0 = (warp - 10) * 128 + lane; x0 < kTile * 8; x0 += 256) {
                 uint4 v[4];
                 uint32_t bad = 0;
@@ -728,7 +761,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
                 for (int u = 0; u < 4; ++u) {
                   const int x = x0 + 32 * u;
                   v[u] = make_uint4(0, 0, 0, 0);
-                  if (x >= first && x < behind) v[u] = ld_shared_v4(base + x * 16);
+                  if (x >= first && x < behind) v[u] = ld_shared_v4(vector_at(x));
                 }
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
@@ -740,14 +773,14 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
                   for (int u = 0; u < 4; ++u) {
                     const int x = x0 + 32 * u;
                     if (x >= first && x < behind)
-                      st_shared_v4(base + x * 16, make_uint4(finite_or_zero(v[u].x), finite_or_zero(v[u].y),
-                                                             finite_or_zero(v[u].z), finite_or_zero(v[u].w)));
+                      st_shared_v4(vector_at(x), make_uint4(finite_or_zero(v[u].x), finite_or_zero(v[u].y),
+                                                            finite_or_zero(v[u].z), finite_or_zero(v[u].w)));
                   }
                 }
                 if (x0 + 96 >= behind) {
 #pragma unroll
                   for (int u = 0; u < 4; ++u)
-                    if (x0 + 32 * u >= behind) st_shared_v4(base + (x0 + 32 * u) * 16, make_uint4(0, 0, 0, 0));
+                    if (x0 + 32 * u >= behind) st_shared_v4(vector_at(x0 + 32 * u), make_uint4(0, 0, 0, 0));
                 }
               }
             }
@@ -800,8 +833,13 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         tmem_wait_ld();
         if ((j + 1) * kTile > all_see) {
           const int limit = sees - j * kTile;
+          if (kPair && p.page_shift == 4) {
 #pragma unroll
-          for (int c = 0; c < kTile; ++c) s[c] = c < limit ? s[c] : -INFINITY;
+            for (int c = 0; c < kTile; ++c) s[c] = tile_key16(c) < limit ? s[c] : -INFINITY;
+          } else {
+#pragma unroll
+            for (int c = 0; c < kTile; ++c) s[c] = c < limit ? s[c] : -INFINITY;
+          }
         }
         float m0 = -INFINITY, m1 = m0, m2 = m0, m3 = m0;
 #pragma unroll
