@@ -59,9 +59,9 @@ int check_rows(const void* table, int64_t stride, const void* lens, int64_t batc
 
 // Launches `kernel` with programmatic stream serialisation (it waits for the
 // kernels before it itself).
-template <typename Params>
-int launch(void (*kernel)(Params), const Params& p, int64_t grid, int threads, size_t smem, int device,
-           void* stream, const char* what) {
+template <typename... Args>
+int launch(void (*kernel)(Args...), int64_t grid, int threads, size_t smem, int device, void* stream,
+           const char* what, Args... args) {
   DeviceGuard guard(device);
   if (guard.error != cudaSuccess) return cuda_fail(guard.error, "cudaSetDevice");
   int sms = 0;
@@ -82,7 +82,7 @@ int launch(void (*kernel)(Params), const Params& p, int64_t grid, int threads, s
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kernel, p);
+  e = cudaLaunchKernelEx(&cfg, kernel, args...);
   if (e != cudaSuccess) return cuda_fail(e, what);
   adb_host::count_launch();
   return ADB_OK;
@@ -121,8 +121,11 @@ int adb_cache_write(const void* k, int64_t k_token_stride, int64_t k_head_stride
   if (!is_aligned(k, 16) || !is_aligned(v, 16) || !is_aligned(k_cache, 16) || !is_aligned(v_cache, 16) ||
       ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7) != 0)
     return fail(ADB_ERR_INVALID_ARGUMENT, "K, V and caches must be 16-byte aligned, strides multiples of 8 elements");
-  const int64_t blocks = (total * kv_heads * (head_dim / 8) + adb::kWriteThreads - 1) / adb::kWriteThreads;
-  if (blocks > INT32_MAX) return fail(ADB_ERR_INVALID_ARGUMENT, "too many elements for one call");
+  // tokens per block: as many as fill its threads' loads, fewer where the GPU would not be filled
+  const int64_t vecs = kv_heads * (head_dim / 8);
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(adb::kWriteThreads, adb::kWriteThreads * adb::kWriteVecs / vecs));
+  const int64_t tokens = std::max<int64_t>(1, std::min<int64_t>(most, total / (2 * 148)));
+  const int64_t blocks = (total + tokens - 1) / tokens;
   adb::WriteParams p;
   p.k = static_cast<const __nv_bfloat16*>(k);
   p.v = static_cast<const __nv_bfloat16*>(v);
@@ -144,7 +147,8 @@ int adb_cache_write(const void* k, int64_t k_token_stride, int64_t k_head_stride
   p.num_blocks = static_cast<int>(num_blocks);
   p.page_shift = shift;
   p.nhd = layout == ADB_PAGED_NHD;
-  return launch(&adb::cache_write_kernel, p, blocks, adb::kWriteThreads, 0, device, stream, "cache write launch");
+  return launch(&adb::cache_write_kernel, blocks, adb::kWriteThreads, 0, device, stream, "cache write launch", p,
+                static_cast<int>(tokens));
 }
 
 int adb_cache_copy_pages(void* k_cache, void* v_cache, const int32_t* src, const int32_t* dst, int64_t count,
@@ -167,7 +171,7 @@ int adb_cache_copy_pages(void* k_cache, void* v_cache, const int32_t* src, const
   p.chunks = static_cast<int>(chunks);
   p.num_blocks = static_cast<int>(num_blocks);
   const int64_t grid = std::min<int64_t>(count * chunks, 148 * 8);
-  return launch(&adb::cache_copy_pages_kernel, p, grid, adb::kCopyThreads, 0, device, stream, "page copy launch");
+  return launch(&adb::cache_copy_pages_kernel, grid, adb::kCopyThreads, 0, device, stream, "page copy launch", p);
 }
 
 int adb_cache_resize(int32_t* block_table, int64_t block_table_stride, const int32_t* seqlens,
@@ -189,8 +193,8 @@ int adb_cache_resize(int32_t* block_table, int64_t block_table_stride, const int
   p.batch = static_cast<int>(batch);
   p.max_blocks = static_cast<int>(max_blocks_per_seq);
   p.num_blocks = static_cast<int>(num_blocks);
-  return launch(&adb::cache_resize_kernel, p, adb::kBookCtas, adb::kBookThreads, batch * sizeof(int), device, stream,
-                "cache resize launch");
+  return launch(&adb::cache_resize_kernel, adb::kBookCtas, adb::kBookThreads, 3 * batch * sizeof(int), device, stream,
+                "cache resize launch", p);
 }
 
 int adb_cache_fork(int32_t* block_table, int64_t block_table_stride, const int32_t* seqlens, int32_t* page_refs,
@@ -204,6 +208,8 @@ int adb_cache_fork(int32_t* block_table, int64_t block_table_stride, const int32
     return fail(ADB_ERR_INVALID_ARGUMENT, "fork needs page_refs, parents, children and its outputs");
   if (forks <= 0 || forks > kMaxRows)
     return fail(ADB_ERR_UNSUPPORTED, "1 to %lld forks per call (got %lld)", (long long)kMaxRows, (long long)forks);
+  if (forks * max_blocks_per_seq > INT32_MAX)
+    return fail(ADB_ERR_INVALID_ARGUMENT, "forks * max_blocks_per_seq must be below 2^31");
   adb::ForkParams p;
   rc = check_pages(page_size, num_blocks, max_blocks_per_seq, &p.page_shift);
   if (rc != ADB_OK) return rc;
@@ -220,8 +226,8 @@ int adb_cache_fork(int32_t* block_table, int64_t block_table_stride, const int32
   p.forks = static_cast<int>(forks);
   p.max_blocks = static_cast<int>(max_blocks_per_seq);
   p.num_blocks = static_cast<int>(num_blocks);
-  return launch(&adb::cache_fork_kernel, p, adb::kBookCtas, adb::kBookThreads, (batch + forks) * sizeof(int), device,
-                stream, "cache fork launch");
+  return launch(&adb::cache_fork_kernel, adb::kBookCtas, adb::kBookThreads, (batch + 2 * forks) * sizeof(int), device,
+                stream, "cache fork launch", p);
 }
 
 int adb_cache_compact(int32_t* block_table, int64_t block_table_stride, const int32_t* seqlens, int32_t* page_refs,
@@ -244,8 +250,8 @@ int adb_cache_compact(int32_t* block_table, int64_t block_table_stride, const in
   p.batch = static_cast<int>(batch);
   p.max_blocks = static_cast<int>(max_blocks_per_seq);
   p.num_blocks = static_cast<int>(num_blocks);
-  return launch(&adb::cache_compact_kernel, p, adb::kBookCtas, adb::kBookThreads, 0, device, stream,
-                "cache compact launch");
+  return launch(&adb::cache_compact_kernel, adb::kBookCtas, adb::kBookThreads, 0, device, stream,
+                "cache compact launch", p);
 }
 
 }  // extern "C"

@@ -12,7 +12,13 @@
 // the table entries that change): it is bound by latency, not by bytes.  Each
 // is therefore ONE launch of ONE cluster of 8 CTAs x 1024 threads, whose steps
 // are separated by cluster barriers and whose prefix sums cross CTAs through
-// distributed shared memory, instead of a chain of kernels.
+// distributed shared memory, instead of a chain of kernels.  What all CTAs need
+// of the rows (lengths, prefix sums) each keeps in its own shared memory, read
+// from global memory once, and a warp keeps the bits of the pages that it
+// counted, so that a step waits for memory as seldom as possible.
+//
+// Every kernel lets the next one start at once: kernels of this library wait
+// (griddepcontrol.wait) before they touch memory, others for the grid's end.
 #pragma once
 
 #include "device_primitives.cuh"
@@ -23,13 +29,18 @@ constexpr int kBookCtas = 8;       // portable cluster size
 constexpr int kBookThreads = 1024;
 constexpr int kBookWarps = kBookThreads / 32;
 constexpr int kBookAllWarps = kBookCtas * kBookWarps;
-constexpr int kBookChunk = 512;    // table entries of a row that one warp handles
+constexpr int kBookChunk = 128;    // table entries of a row that one warp handles
 
 // ------------------------------------------------------------ cluster
 // Release/acquire at cluster scope: orders global and shared accesses of the
 // cluster's threads before it against those after it.
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// No CTA of the cluster leaves before all have come here; orders no memory.
+__device__ __forceinline__ void cluster_leave() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -62,7 +73,6 @@ struct BookShared {
   int total[2];    // of this CTA, read by its peers (one per counting pass)
   int before;      // sum of the totals of the CTAs before this one
   int all;         // sum of every CTA's total
-  int flag;        // read by its peers
 };
 
 // Exclusive prefix of v over the block; *sum gets the block's total.
@@ -89,18 +99,42 @@ __device__ __forceinline__ Region page_region(int num_blocks) {
   return {static_cast<int>(lo < num_blocks ? lo : num_blocks), static_cast<int>(hi < num_blocks ? hi : num_blocks)};
 }
 
-// Counts the pages that `pred` holds for: returns how many are in regions
-// before this warp's; sh.all is the count over the pool.  Ends with a cluster
-// barrier, so what was written before the call is visible to the cluster.
-template <int kPass, typename Pred>
-__device__ __forceinline__ int count_pages(const Region& r, BookShared& sh, Pred pred) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int mine = 0;
-#pragma unroll 4
-  for (int p = r.lo; p < r.hi; p += 32) {
-    const bool hit = p + lane < r.hi && pred(p + lane);
-    mine += __popc(__ballot_sync(0xffffffffu, hit));
+// The pages of a warp's region for which a predicate holds: the bits of pages
+// lo + 32 n .. + 31 are in lane n of `bits`, read again where a region has more
+// than 32 x 32 pages.
+struct PageBits {
+  Region r;
+  uint32_t bits;
+  int count;
+};
+
+template <typename Pred>
+__device__ __forceinline__ PageBits find_pages(int num_blocks, Pred pred) {
+  const int lane = threadIdx.x & 31;
+  PageBits b{page_region(num_blocks), 0u, 0};
+#pragma unroll 8
+  for (int p = b.r.lo; p < b.r.hi; p += 32) {
+    const bool hit = p + lane < b.r.hi && pred(p + lane);
+    const unsigned hits = __ballot_sync(0xffffffffu, hit);
+    if (lane == (p - b.r.lo) >> 5) b.bits = hits;
+    b.count += __popc(hits);
   }
+  return b;
+}
+
+template <typename Pred>
+__device__ __forceinline__ unsigned page_bits(const PageBits& b, int at, Pred pred) {
+  const int n = (at - b.r.lo) >> 5, lane = threadIdx.x & 31;
+  if (n < 32) return __shfl_sync(0xffffffffu, b.bits, n);
+  return __ballot_sync(0xffffffffu, at + lane < b.r.hi && pred(at + lane));
+}
+
+// Sums a warp's count over the cluster: returns the sum over the warps before
+// this one; sh.all is the total.  Ends with a cluster barrier, so what was
+// written before the call is visible to the cluster.
+template <int kPass>
+__device__ __forceinline__ int cluster_prefix(int mine, BookShared& sh) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   __syncthreads();
   if (lane == 0) sh.warp[warp] = mine;
   __syncthreads();
@@ -121,16 +155,8 @@ __device__ __forceinline__ int count_pages(const Region& r, BookShared& sh, Pred
   return sh.before + sh.warp[warp] - mine;
 }
 
-// Whether any CTA of the cluster raised sh.flag before its last barrier.
-__device__ __forceinline__ bool any_flag(BookShared& sh) {
-  const int lane = threadIdx.x & 31;
-  const int f = lane < kBookCtas ? peer_shared(&sh.flag, lane) : 0;
-  return __any_sync(0xffffffffu, f != 0);
-}
-
-// Last index i of [0, n) with prefix[i] <= rank (prefix ascending, prefix[0] = 0).
-__device__ __forceinline__ int last_at_most(const int* prefix, int n, int rank) {
-  int lo = 0, hi = n - 1;
+// Last index i of [lo, hi] with prefix[i] <= rank (prefix ascending, prefix[lo] <= rank).
+__device__ __forceinline__ int last_at_most(const int* prefix, int lo, int hi, int rank) {
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (prefix[mid] <= rank)
@@ -139,6 +165,30 @@ __device__ __forceinline__ int last_at_most(const int* prefix, int n, int rank) 
       hi = mid - 1;
   }
   return lo;
+}
+
+// Entries [from, to) of the rows in units of kBookChunk, a warp per unit: each
+// lane looks whether there is work in one unit, then the warp does those units.
+// range(row, from, to); work(row, from, to) with from < to inside one unit.
+template <typename Range, typename Work>
+__device__ __forceinline__ void each_chunk(int rows, int max_blocks, Range range, Work work) {
+  const int lane = threadIdx.x & 31;
+  const int chunks = (max_blocks + kBookChunk - 1) / kBookChunk, units = rows * chunks;
+  for (int u0 = cluster_rank() * kBookWarps + (threadIdx.x >> 5); u0 < units; u0 += 32 * kBookAllWarps) {
+    const int u = u0 + lane * kBookAllWarps;
+    int row = 0, from = 0, to = 0;
+    if (u < units) {
+      row = u / chunks;
+      const int c = (u - row * chunks) * kBookChunk;
+      range(row, from, to);
+      from = max(from, c);
+      to = min(to, c + kBookChunk);
+    }
+    for (unsigned todo = __ballot_sync(0xffffffffu, from < to); todo != 0; todo &= todo - 1) {
+      const int l = __ffs(todo) - 1;
+      work(__shfl_sync(0xffffffffu, row, l), __shfl_sync(0xffffffffu, from, l), __shfl_sync(0xffffffffu, to, l));
+    }
+  }
 }
 
 __device__ __forceinline__ int clamp_len(int n, int cap) { return n < 0 ? 0 : (n > cap ? cap : n); }
@@ -158,121 +208,144 @@ struct ResizeParams {
 template <typename Range>
 __device__ __forceinline__ void let_go(const ResizeParams& p, Range range) {
   const int lane = threadIdx.x & 31;
-  const int64_t chunks = (p.max_blocks + kBookChunk - 1) / kBookChunk;
-  for (int64_t u = cluster_rank() * kBookWarps + (threadIdx.x >> 5); u < chunks * p.batch; u += kBookAllWarps) {
-    const int b = static_cast<int>(u / chunks), c = static_cast<int>(u % chunks) * kBookChunk;
-    int from, to;
-    range(b, from, to);
-    from = max(from, c);
-    to = min(to, c + kBookChunk);
+  each_chunk(p.batch, p.max_blocks, range, [&](int b, int from, int to) {
     int32_t* row = p.table + b * p.stride;
-#pragma unroll 4
-    for (int j = from + lane; j < to; j += 32) {
-      const int page = row[j];
-      row[j] = -1;
-      if (static_cast<unsigned>(page) < static_cast<unsigned>(p.num_blocks)) {
-        if (atomicSub(&p.refs[page], 1) > 0) continue;
-        atomicAdd(&p.refs[page], 1);  // nobody held it: the tables disagree
+    int page[kBookChunk / 32], left[kBookChunk / 32];
+#pragma unroll
+    for (int x = 0; x < kBookChunk / 32; ++x) {
+      const int j = from + lane + 32 * x;
+      page[x] = j < to ? row[j] : -1;
+    }
+#pragma unroll
+    for (int x = 0; x < kBookChunk / 32; ++x) {
+      const int j = from + lane + 32 * x;
+      left[x] = 1;
+      if (j < to) {
+        row[j] = -1;
+        left[x] = static_cast<unsigned>(page[x]) < static_cast<unsigned>(p.num_blocks) ? atomicSub(&p.refs[page[x]], 1) : 0;
       }
+    }
+#pragma unroll
+    for (int x = 0; x < kBookChunk / 32; ++x) {
+      if (left[x] > 0) continue;  // no page, or nobody held it: the tables disagree
+      if (static_cast<unsigned>(page[x]) < static_cast<unsigned>(p.num_blocks)) atomicAdd(&p.refs[page[x]], 1);
       atomicOr(&g_adb_error_flag, kErrCachePage);
     }
-  }
+  });
 }
 
 // Steps: rows that end let their pages go; cuts are judged (refused where the
 // page that stays partly used is held by another row, whose tokens the row's
 // next ones would overwrite) and then made; the free pages are counted and
-// handed out, lowest first, to the growing rows in row order.
+// handed out, lowest first, to the growing rows in row order.  Steps that no
+// row asks for are skipped.
 __global__ void __cluster_dims__(kBookCtas, 1, 1) __launch_bounds__(kBookThreads)
     cache_resize_kernel(const ResizeParams p) {
-  extern __shared__ int prefix[];  // [batch]: pages needed by the rows before
+  extern __shared__ int resize_smem[];
+  int* prefix = resize_smem;             // [batch]: pages needed by the rows before
+  int* olds = resize_smem + p.batch;     // [batch]: lengths before
+  int* wants = resize_smem + 2 * p.batch;  // [batch]: lengths asked for; refused: as before
   __shared__ BookShared sh;
   const int tid = threadIdx.x, lane = tid & 31;
+  const int all_tid = cluster_rank() * kBookThreads + tid;
   const int mask = (1 << p.page_shift) - 1;
   const int cap = p.max_blocks << p.page_shift;
   const auto pages = [&](int n) { return static_cast<int>((static_cast<unsigned>(n) + mask) >> p.page_shift); };
-  if (tid == 0) sh.flag = 0;
+  griddep_launch_dependents();
   griddep_wait();
 
-  let_go(p, [&](int b, int& from, int& to) {
-    from = 0;
-    to = p.want[b] == 0 ? pages(clamp_len(p.lens[b], cap)) : 0;
-  });
-  cluster_sync();
-
-  for (int b = cluster_rank() * kBookThreads + tid; b < p.batch; b += kBookCtas * kBookThreads) {
-    const int old = clamp_len(p.lens[b], cap), w = p.want[b];
-    int after = old;
-    bool refused = w < 0 || w > cap;
-    if (w == 0) {
-      after = 0;
-    } else if (!refused && w < old) {
-      if (w & mask) {
-        const int page = p.table[b * p.stride + (w >> p.page_shift)];
-        refused = static_cast<unsigned>(page) < static_cast<unsigned>(p.num_blocks) && p.refs[page] > 1;
-      }
-      if (!refused) {
-        after = w;
-        sh.flag = 1;
-      }
-    }
-    p.lens_out[b] = after;
-    if (refused) atomicOr(&g_adb_error_flag, kErrCacheRefused);
-  }
-  // the pages that each growing row needs, and those of the rows before it
-  int needed = 0;
+  int needed = 0, drops = 0, cuts = 0;
   for (int base = 0; base < p.batch; base += kBookThreads) {
     const int b = base + tid;
     int need = 0;
     if (b < p.batch) {
-      const int old = clamp_len(p.lens[b], cap), w = p.want[b];
-      if (w > old && w <= cap) need = pages(w) - pages(old);
+      const int old = clamp_len(p.lens[b], cap);
+      int w = p.want[b];
+      if (w < 0 || w > cap) {
+        w = old;
+        if (cluster_rank() == 0) atomicOr(&g_adb_error_flag, kErrCacheRefused);
+      }
+      olds[b] = old;
+      wants[b] = w;
+      if (w > old) need = pages(w) - pages(old);
+      drops |= w == 0 && old > 0;
+      cuts |= w > 0 && w < old;
     }
     int sum;
     const int before = block_exclusive(need, sh, &sum);
     if (b < p.batch) prefix[b] = needed + before;
     needed += sum;
   }
-  cluster_sync();
-  if (any_flag(sh)) {
+  drops = __syncthreads_or(drops);
+  cuts = __syncthreads_or(cuts);
+  if (drops) {
     let_go(p, [&](int b, int& from, int& to) {
-      const int old = clamp_len(p.lens[b], cap), w = p.want[b];
-      const bool cut = w > 0 && w < old && p.lens_out[b] == w;
-      from = cut ? pages(w) : 0;
-      to = cut ? pages(old) : 0;
+      from = 0;
+      to = wants[b] == 0 ? pages(olds[b]) : 0;
+    });
+    cluster_sync();
+  }
+  if (cuts) {
+    // every CTA judges for itself, and none changes a count until all have
+    bool refused = false;
+    for (int b = tid; b < p.batch; b += kBookThreads) {
+      const int old = olds[b], w = wants[b];
+      if (w == 0 || w >= old || (w & mask) == 0) continue;
+      const int page = p.table[b * p.stride + (w >> p.page_shift)];
+      if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_blocks) || __ldcg(&p.refs[page]) <= 1) continue;
+      wants[b] = old;
+      refused = true;
+    }
+    if (refused && cluster_rank() == 0) atomicOr(&g_adb_error_flag, kErrCacheRefused);
+    cluster_sync();
+    let_go(p, [&](int b, int& from, int& to) {
+      const bool cut = wants[b] > 0 && wants[b] < olds[b];
+      from = cut ? pages(wants[b]) : 0;
+      to = cut ? pages(olds[b]) : 0;
     });
     cluster_sync();
   }
 
-  const Region r = page_region(p.num_blocks);
-  int rank = count_pages<0>(r, sh, [&](int page) { return p.refs[page] == 0; });
-  const int free_pages = sh.all;
-  for (int at = r.lo; at < r.hi && rank < needed; at += 32) {
-    const int page = at + lane;
-    const bool hit = page < r.hi && p.refs[page] == 0;
-    const unsigned hits = __ballot_sync(0xffffffffu, hit);
-    const int mine = rank + __popc(hits & ((1u << lane) - 1));
-    if (hit && mine < needed) {
-      const int b = last_at_most(prefix, p.batch, mine);
-      const int first = pages(clamp_len(p.lens[b], cap)), last = pages(p.want[b]);
-      if (prefix[b] + (last - first) <= free_pages) {
-        p.table[b * p.stride + first + mine - prefix[b]] = page;
-        p.refs[page] = 1;
+  const auto is_free = [&](int page) { return __ldcg(&p.refs[page]) == 0; };
+  if (needed > 0) {  // (the same in all CTAs)
+    const PageBits free = find_pages(p.num_blocks, is_free);
+    int rank = cluster_prefix<0>(free.count, sh);
+    // Consecutive ranks are mostly of one row: the warp keeps the row of its last
+    // one, and each lane searches only where a row ends among the 32 pages.
+    int row = rank < needed ? last_at_most(prefix, 0, p.batch - 1, rank) : 0;
+    for (int at = free.r.lo; at < free.r.hi && rank < needed; at += 32) {
+      const unsigned hits = page_bits(free, at, is_free);
+      if (hits == 0) continue;
+      const int mine = rank + __popc(hits & ((1u << lane) - 1));
+      const int row1 = row + 1 == p.batch || prefix[row + 1] > rank + __popc(hits) - 1
+                           ? row
+                           : last_at_most(prefix, row, p.batch - 1, rank + __popc(hits) - 1);
+      const int row0 = row;
+      row = row1;
+      if ((hits >> lane & 1) && mine < needed) {
+        const int b = last_at_most(prefix, row0, row1, mine);
+        const int first = pages(olds[b]), last = pages(wants[b]);
+        if (prefix[b] + (last - first) <= sh.all) {
+          p.table[b * p.stride + first + mine - prefix[b]] = at + lane;
+          p.refs[at + lane] = 1;
+        }
+      }
+      rank += __popc(hits);
+    }
+  }
+  for (int b = all_tid; b < p.batch; b += kBookCtas * kBookThreads) {
+    const int old = olds[b];
+    int after = wants[b];
+    if (after > old) {
+      const int need = pages(after) - pages(old);
+      if (need > 0 && prefix[b] + need > sh.all) {
+        after = old;
+        atomicOr(&g_adb_error_flag, kErrCacheFull);
       }
     }
-    rank += __popc(hits);
+    p.lens_out[b] = after;
   }
-  for (int b = cluster_rank() * kBookThreads + tid; b < p.batch; b += kBookCtas * kBookThreads) {
-    const int old = clamp_len(p.lens[b], cap), w = p.want[b];
-    if (w <= old || w > cap) continue;
-    const int need = pages(w) - pages(old);
-    if (need == 0 || prefix[b] + need <= free_pages)
-      p.lens_out[b] = w;
-    else
-      atomicOr(&g_adb_error_flag, kErrCacheFull);
-  }
-  griddep_launch_dependents();
-  cluster_sync();  // no CTA leaves while a peer may read its shared memory
+  cluster_leave();  // a peer may still read this CTA's shared memory
 }
 
 // ------------------------------------------------------------ fork
@@ -291,98 +364,102 @@ struct ForkParams {
 
 // A child shares its parent's full pages (they no longer change) and gets a
 // page of its own for the partly filled last one.  Each CTA keeps, redundantly,
-// which fork a row is the child of (the first that names it) and the prefix
-// sum of the pages needed.
+// which fork a row is the child of (the first that names it), the tokens that
+// each fork takes over and the prefix sum of the pages needed.
 __global__ void __cluster_dims__(kBookCtas, 1, 1) __launch_bounds__(kBookThreads)
     cache_fork_kernel(const ForkParams p) {
   extern __shared__ int fork_smem[];
-  int* prefix = fork_smem;            // [forks]
-  int* claim = fork_smem + p.forks;   // [batch]: first fork that names the row as its child
+  int* prefix = fork_smem;               // [forks]
+  int* tokens = fork_smem + p.forks;     // [forks]: -1 where refused
+  int* claim = fork_smem + 2 * p.forks;  // [batch]: first fork that names the row as its child
   __shared__ BookShared sh;
   const int tid = threadIdx.x, lane = tid & 31;
+  const int all_tid = cluster_rank() * kBookThreads + tid;
   const int mask = (1 << p.page_shift) - 1;
   const int cap = p.max_blocks << p.page_shift;
+  const unsigned rows = static_cast<unsigned>(p.batch);
   for (int b = tid; b < p.batch; b += kBookThreads) claim[b] = INT32_MAX;
   __syncthreads();
+  griddep_launch_dependents();
   griddep_wait();
+  // the pages' loads do not depend on the forks': issued first
+  const auto is_free = [&](int page) { return __ldcg(&p.refs[page]) == 0; };
+  const PageBits free = find_pages(p.num_blocks, is_free);
   for (int i = tid; i < p.forks; i += kBookThreads) {
     const int c = p.children[i];
-    if (static_cast<unsigned>(c) < static_cast<unsigned>(p.batch)) atomicMin(&claim[c], i);
+    if (static_cast<unsigned>(c) < rows) atomicMin(&claim[c], i);
   }
   __syncthreads();
-  // -1: refused; otherwise the tokens that the child takes over
-  const auto tokens = [&](int i) {
-    const int a = p.parents[i], c = p.children[i];
-    const unsigned rows = static_cast<unsigned>(p.batch);
-    if (static_cast<unsigned>(a) >= rows || static_cast<unsigned>(c) >= rows) return -1;
-    if (claim[c] != i || p.lens[c] != 0) return -1;
-    return clamp_len(p.lens[a], cap);
-  };
   int needed = 0;
   for (int base = 0; base < p.forks; base += kBookThreads) {
     const int i = base + tid;
-    const int n = i < p.forks ? tokens(i) : 0;
+    int n = -1;
+    if (i < p.forks) {
+      const int a = p.parents[i], c = p.children[i];
+      if (static_cast<unsigned>(a) < rows && static_cast<unsigned>(c) < rows && claim[c] == i && p.lens[c] == 0)
+        n = clamp_len(p.lens[a], cap);
+      tokens[i] = n;
+      if (n < 0 && cluster_rank() == 0) atomicOr(&g_adb_error_flag, kErrCacheRefused);
+    }
     int sum;
     const int before = block_exclusive(n > 0 && (n & mask) != 0, sh, &sum);
     if (i < p.forks) prefix[i] = needed + before;
     needed += sum;
   }
-  const Region r = page_region(p.num_blocks);
-  int rank = count_pages<0>(r, sh, [&](int page) { return p.refs[page] == 0; });
+  int rank = cluster_prefix<0>(free.count, sh);
   const int free_pages = sh.all;
-  // every CTA has counted (the barrier in count_pages): the counts may change now
+  // every CTA has counted (the barrier in cluster_prefix): the counts may change now
   const auto granted = [&](int i, int n) { return n >= 0 && ((n & mask) == 0 || prefix[i] < free_pages); };
 
-  for (int at = r.lo; at < r.hi && rank < needed; at += 32) {
-    const int page = at + lane;
-    const bool hit = page < r.hi && p.refs[page] == 0;
-    const unsigned hits = __ballot_sync(0xffffffffu, hit);
+  // (a region of more pages than its bits hold is read again: only pages that were live change their count)
+  for (int at = free.r.lo; at < free.r.hi && rank < needed; at += 32) {
+    const unsigned hits = page_bits(free, at, is_free);
     const int mine = rank + __popc(hits & ((1u << lane) - 1));
-    if (hit && mine < needed) {
+    if ((hits >> lane & 1) && mine < needed) {
       // forks without a copy repeat the next prefix: the last one at `mine` is the one that needs it
-      const int i = last_at_most(prefix, p.forks, mine);
-      const int a = p.parents[i], full = clamp_len(p.lens[a], cap) >> p.page_shift;
-      p.src[i] = p.table[a * p.stride + full];
-      p.dst[i] = page;
-      p.table[p.children[i] * p.stride + full] = page;
-      p.refs[page] = 1;
+      const int i = last_at_most(prefix, 0, p.forks - 1, mine);
+      const int full = tokens[i] >> p.page_shift;
+      p.src[i] = p.table[p.parents[i] * p.stride + full];
+      p.dst[i] = at + lane;
+      p.table[p.children[i] * p.stride + full] = at + lane;
+      p.refs[at + lane] = 1;
     }
     rank += __popc(hits);
   }
 
-  const int all_tid = cluster_rank() * kBookThreads + tid;
   for (int i = all_tid; i < p.forks; i += kBookCtas * kBookThreads) {
-    const int n = tokens(i);
-    const bool copies = granted(i, n) && (n & mask) != 0;
-    if (!copies) p.src[i] = p.dst[i] = -1;
-    if (n < 0) atomicOr(&g_adb_error_flag, kErrCacheRefused);
+    const int n = tokens[i];
+    if (!granted(i, n) || (n & mask) == 0) p.src[i] = p.dst[i] = -1;
     if (n >= 0 && !granted(i, n)) atomicOr(&g_adb_error_flag, kErrCacheFull);
   }
   for (int b = all_tid; b < p.batch; b += kBookCtas * kBookThreads) {
     const int i = claim[b];
-    const int n = i < p.forks ? tokens(i) : -1;
+    const int n = i < p.forks ? tokens[i] : -1;
     p.lens_out[b] = n >= 0 && granted(i, n) ? n : p.lens[b];
   }
-  const int64_t chunks = (p.max_blocks + kBookChunk - 1) / kBookChunk;
-  for (int64_t u = cluster_rank() * kBookWarps + (tid >> 5); u < chunks * p.forks; u += kBookAllWarps) {
-    const int i = static_cast<int>(u / chunks), c = static_cast<int>(u % chunks) * kBookChunk;
-    const int n = tokens(i);
-    if (!granted(i, n)) continue;
-    const int to = min(n >> p.page_shift, c + kBookChunk);
-    const int32_t* from_row = p.table + p.parents[i] * p.stride;
-    int32_t* to_row = p.table + p.children[i] * p.stride;
-#pragma unroll 4
-    for (int j = c + lane; j < to; j += 32) {
-      const int page = from_row[j];
-      to_row[j] = page;
-      if (static_cast<unsigned>(page) < static_cast<unsigned>(p.num_blocks))
-        atomicAdd(&p.refs[page], 1);
-      else
-        atomicOr(&g_adb_error_flag, kErrCachePage);
-    }
-  }
-  griddep_launch_dependents();
-  cluster_sync();
+  each_chunk(
+      p.forks, p.max_blocks,
+      [&](int i, int& from, int& to) {
+        const int n = tokens[i];
+        from = 0;
+        to = granted(i, n) ? n >> p.page_shift : 0;
+      },
+      [&](int i, int from, int to) {
+        const int32_t* from_row = p.table + p.parents[i] * p.stride;
+        int32_t* to_row = p.table + p.children[i] * p.stride;
+#pragma unroll
+        for (int x = 0; x < kBookChunk / 32; ++x) {
+          const int j = from + lane + 32 * x;
+          if (j >= to) continue;
+          const int page = from_row[j];
+          to_row[j] = page;
+          if (static_cast<unsigned>(page) < static_cast<unsigned>(p.num_blocks))
+            atomicAdd(&p.refs[page], 1);
+          else
+            atomicOr(&g_adb_error_flag, kErrCachePage);
+        }
+      });
+  cluster_leave();
 }
 
 // ------------------------------------------------------------ compact
@@ -406,58 +483,77 @@ __global__ void __cluster_dims__(kBookCtas, 1, 1) __launch_bounds__(kBookThreads
   const int tid = threadIdx.x, lane = tid & 31;
   const int mask = (1 << p.page_shift) - 1;
   const int cap = p.max_blocks << p.page_shift;
+  griddep_launch_dependents();
   griddep_wait();
-  const Region r = page_region(p.num_blocks);
-  int before = count_pages<0>(r, sh, [&](int page) { return p.refs[page] > 0; });
+  const auto is_live = [&](int page) { return __ldcg(&p.refs[page]) > 0; };
+  const PageBits held = find_pages(p.num_blocks, is_live);
+  int before = cluster_prefix<0>(held.count, sh);
   const int live = sh.all;
   // live pages below `live` stay; their count ranks the others
-  count_pages<1>(r, sh, [&](int page) { return page < live && p.refs[page] > 0; });
+  int below = 0;
+  for (int at = held.r.lo; at < held.r.hi && at < live; at += 32) {
+    const unsigned bits = page_bits(held, at, is_live);
+    below += __popc(live - at >= 32 ? bits : bits & ((1u << (live - at)) - 1));
+  }
+  cluster_prefix<1>(below, sh);
   const int stay = sh.all, moves = live - stay;
-  for (int at = r.lo; at < r.hi; at += 32) {
+  for (int at = held.r.lo; at < held.r.hi; at += 32) {
     const int page = at + lane;
-    const bool in = page < r.hi, held = in && p.refs[page] > 0;
-    const unsigned hits = __ballot_sync(0xffffffffu, held);
-    const int mine = before + __popc(hits & ((1u << lane) - 1));  // live pages before this one
-    if (in && page < live && !held) p.dst[page - mine] = page;
-    if (in && page >= live) {
-      p.remap[page] = held ? mine - stay : -1;
-      if (held) p.src[mine - stay] = page;
+    const unsigned bits = page_bits(held, at, is_live);
+    const bool mine_held = bits >> lane & 1;
+    const int mine = before + __popc(bits & ((1u << lane) - 1));  // live pages before this one
+    if (page < held.r.hi) {
+      if (page >= live) {
+        p.remap[page] = mine_held ? mine - stay : -1;
+        if (mine_held) p.src[mine - stay] = page;
+      } else if (!mine_held) {
+        p.dst[page - mine] = page;
+      }
     }
-    before += __popc(hits);
+    before += __popc(bits);
   }
   cluster_sync();
   const int all_tid = cluster_rank() * kBookThreads + tid;
   for (int i = all_tid; i < p.num_blocks / 2; i += kBookCtas * kBookThreads) {
     if (i < moves) {
-      const int from = p.src[i], to = p.dst[i];
-      p.refs[to] = p.refs[from];
+      const int from = __ldcg(&p.src[i]), to = __ldcg(&p.dst[i]);
+      p.refs[to] = __ldcg(&p.refs[from]);
       p.refs[from] = 0;
     } else {
       p.src[i] = p.dst[i] = -1;
     }
   }
-  const int64_t chunks = (p.max_blocks + kBookChunk - 1) / kBookChunk;
-  for (int64_t u = cluster_rank() * kBookWarps + (tid >> 5); u < chunks * p.batch; u += kBookAllWarps) {
-    const int b = static_cast<int>(u / chunks), c = static_cast<int>(u % chunks) * kBookChunk;
-    const int held = static_cast<int>((static_cast<unsigned>(clamp_len(p.lens[b], cap)) + mask) >> p.page_shift);
-    const int to = min(held, c + kBookChunk);
-    int32_t* row = p.table + b * p.stride;
-#pragma unroll 4
-    for (int j = c + lane; j < to; j += 32) {
-      const int page = row[j];
-      if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_blocks)) {
-        atomicOr(&g_adb_error_flag, kErrCachePage);
-      } else if (page >= live) {
-        const int i = p.remap[page];
-        if (i >= 0)
-          row[j] = p.dst[i];
-        else
-          atomicOr(&g_adb_error_flag, kErrCachePage);  // a page that refs calls free
-      }
-    }
-  }
-  griddep_launch_dependents();
-  cluster_sync();
+  each_chunk(
+      p.batch, p.max_blocks,
+      [&](int b, int& from, int& to) {
+        from = 0;
+        to = static_cast<int>((static_cast<unsigned>(clamp_len(p.lens[b], cap)) + mask) >> p.page_shift);
+      },
+      [&](int b, int from, int to) {
+        int32_t* row = p.table + b * p.stride;
+        int page[kBookChunk / 32], move[kBookChunk / 32];
+#pragma unroll
+        for (int x = 0; x < kBookChunk / 32; ++x) page[x] = from + lane + 32 * x < to ? row[from + lane + 32 * x] : 0;
+#pragma unroll
+        for (int x = 0; x < kBookChunk / 32; ++x) {
+          const bool in = static_cast<unsigned>(page[x]) < static_cast<unsigned>(p.num_blocks);
+          move[x] = -2;  // stays
+          if (!in)
+            move[x] = -1;
+          else if (page[x] >= live)
+            move[x] = __ldcg(&p.remap[page[x]]);  // -1: a page that refs calls free
+        }
+#pragma unroll
+        for (int x = 0; x < kBookChunk / 32; ++x) {
+          const int j = from + lane + 32 * x;
+          if (j >= to || move[x] == -2) continue;
+          if (move[x] >= 0)
+            row[j] = __ldcg(&p.dst[move[x]]);
+          else
+            atomicOr(&g_adb_error_flag, kErrCachePage);
+        }
+      });
+  cluster_leave();
 }
 
 // ------------------------------------------------------------ page copies
@@ -480,6 +576,7 @@ constexpr int kCopyVecs = 1024;  // of K and of V: 16 KB each per unit of work
 __global__ void __launch_bounds__(kCopyThreads) cache_copy_pages_kernel(const CopyParams p) {
   const int lane = threadIdx.x & 31;
   const int64_t units = p.count * p.chunks;
+  griddep_launch_dependents();
   griddep_wait();
   for (int64_t base = blockIdx.x; base < units; base += 32 * static_cast<int64_t>(gridDim.x)) {
     const int64_t u = base + lane * static_cast<int64_t>(gridDim.x);
@@ -536,47 +633,81 @@ struct WriteParams {
   int batch, heads, dim, max_blocks, num_blocks, page_shift, nhd;
 };
 constexpr int kWriteThreads = 256;
+constexpr int kWriteVecs = 2;         // of K and of V per thread
+constexpr int kWriteRows = 2048;      // rows whose offsets a block keeps in shared memory
 
-// One thread moves one 16-byte vector of K and the same one of V.  The source
-// loads do not depend on the place, so they are issued first and the search
-// for the token's row runs in their shadow.
-__global__ void __launch_bounds__(kWriteThreads) cache_write_kernel(const WriteParams p) {
-  const int head_vecs = p.dim >> 3;
-  const int vecs = p.heads * head_vecs;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kWriteThreads + threadIdx.x;
-  griddep_wait();
-  if (i >= p.total * vecs) return;
-  const int64_t t = i / vecs;
-  const int x = static_cast<int>(i - t * vecs);
-  const int head = x / head_vecs, e = (x - head * head_vecs) * 8;
-  const uint4 kv = __ldcs(reinterpret_cast<const uint4*>(p.k + t * p.k_token + head * p.k_head + e));
-  const uint4 vv = __ldcs(reinterpret_cast<const uint4*>(p.v + t * p.v_token + head * p.v_head + e));
-  // last row whose tokens start at or before t
-  int lo = 0, hi = p.batch - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (p.cu[mid] <= t)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  const int64_t first = p.cu[lo];
-  if (t < first || t >= p.cu[lo + 1]) return;  // padding behind the last row
-  const int64_t pos = p.starts[lo] + (t - first);
-  const int64_t j = pos >> p.page_shift;
-  int page = -1;
-  if (pos >= 0 && j < p.max_blocks) page = p.table[lo * p.stride + j];
-  if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_blocks)) {
-    if (x == 0) atomicOr(&g_adb_error_flag, kErrCachePage);
-    return;
-  }
-  const int64_t slot = pos & ((int64_t(1) << p.page_shift) - 1);
+// A block takes `tokens` tokens.  The source loads do not depend on the places,
+// so they are issued first; meanwhile a thread per token finds its row, in
+// offsets that the block has read at once, and its page.
+__global__ void __launch_bounds__(kWriteThreads) cache_write_kernel(const WriteParams p, const int tokens) {
+  __shared__ int cu[kWriteRows + 1], starts[kWriteRows];
+  __shared__ int64_t place[kWriteThreads];  // element offset of head 0's row; -1: not written
+  const int tid = threadIdx.x;
+  const int head_vecs = p.dim >> 3, vecs = p.heads * head_vecs;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * tokens;
+  const int n = static_cast<int>(min(static_cast<int64_t>(tokens), p.total - first));
   const int64_t page_size = int64_t(1) << p.page_shift;
-  const int64_t row = p.nhd ? (page * page_size + slot) * p.heads + head
-                            : (static_cast<int64_t>(page) * p.heads + head) * page_size + slot;
-  const int64_t at = row * p.dim + e;
-  *reinterpret_cast<uint4*>(p.k_cache + at) = kv;
-  *reinterpret_cast<uint4*>(p.v_cache + at) = vv;
+  const int64_t head_step = p.nhd ? p.dim : page_size * p.dim;
+  griddep_launch_dependents();
+  griddep_wait();
+  const bool local = p.batch <= kWriteRows;
+  if (local)
+    for (int b = tid; b <= p.batch; b += kWriteThreads) {
+      cu[b] = p.cu[b];
+      if (b < p.batch) starts[b] = p.starts[b];
+    }
+  for (int base = 0; base < n * vecs; base += kWriteThreads * kWriteVecs) {
+    uint4 k[kWriteVecs], v[kWriteVecs];
+#pragma unroll
+    for (int x = 0; x < kWriteVecs; ++x) {
+      const int i = base + tid + x * kWriteThreads;
+      if (i >= n * vecs) continue;
+      const int t = i / vecs, r = i - t * vecs, head = r / head_vecs, e = (r - head * head_vecs) * 8;
+      k[x] = __ldcs(reinterpret_cast<const uint4*>(p.k + (first + t) * p.k_token + head * p.k_head + e));
+      v[x] = __ldcs(reinterpret_cast<const uint4*>(p.v + (first + t) * p.v_token + head * p.v_head + e));
+    }
+    if (base == 0) {
+      __syncthreads();
+      if (tid < n) {
+        const int64_t t = first + tid;
+        const int* offsets = local ? cu : p.cu;
+        // last row whose tokens start at or before t
+        int lo = 0, hi = p.batch - 1;
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (offsets[mid] <= t)
+            lo = mid;
+          else
+            hi = mid - 1;
+        }
+        int64_t at = -1;
+        if (t >= offsets[lo] && t < offsets[lo + 1]) {  // otherwise padding behind the last row
+          const int64_t pos = static_cast<int64_t>(local ? starts[lo] : p.starts[lo]) + (t - offsets[lo]), j = pos >> p.page_shift;
+          int page = -1;
+          if (pos >= 0 && j < p.max_blocks) page = p.table[lo * p.stride + j];
+          if (static_cast<unsigned>(page) < static_cast<unsigned>(p.num_blocks)) {
+            const int64_t slot = pos & (page_size - 1);
+            at = p.nhd ? (page * page_size + slot) * p.heads * p.dim
+                       : (static_cast<int64_t>(page) * p.heads * page_size + slot) * p.dim;
+          } else {
+            atomicOr(&g_adb_error_flag, kErrCachePage);
+          }
+        }
+        place[tid] = at;
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int x = 0; x < kWriteVecs; ++x) {
+      const int i = base + tid + x * kWriteThreads;
+      if (i >= n * vecs) continue;
+      const int t = i / vecs, r = i - t * vecs, head = r / head_vecs, e = (r - head * head_vecs) * 8;
+      if (place[t] < 0) continue;
+      const int64_t at = place[t] + head * head_step + e;
+      *reinterpret_cast<uint4*>(p.k_cache + at) = k[x];
+      *reinterpret_cast<uint4*>(p.v_cache + at) = v[x];
+    }
+  }
 }
 
 }  // namespace adb
