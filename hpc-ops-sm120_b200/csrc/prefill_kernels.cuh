@@ -340,8 +340,10 @@ __device__ __forceinline__ void find_work(const PrefillParams& p, PrefillPlan& p
   w.parts = 1;
   w.part = w.slot = w.join = 0;
   if (index >= plan.units * p.kv_heads) return;
-  const int heads0 = index / (plan.units * p.head_group) * p.head_group;
-  const int heads = min(p.head_group, p.kv_heads - heads0);
+  // (a group has to fill the GPU several times over: its last units leave SMs idle)
+  const int group = plan.units * p.head_group >= 4 * p.sms ? p.head_group : p.kv_heads;
+  const int heads0 = index / (plan.units * group) * group;
+  const int heads = min(group, p.kv_heads - heads0);
   const int at = index - heads0 * plan.units;
   w.head = heads0 + at % heads;
   int pair;
@@ -525,7 +527,6 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       int index = blockIdx.x;
       bool go = true;
       for (int asked = 0; go; ++asked) {
-        if (lane == 0) ask_next(smem_u32(&sh.next), smem_u32(&sh.next_full));
         PrefillWork w;
         find_work(p, plan, index, w);
         w.pad_head = pad_head;
@@ -560,7 +561,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         const int ahead = 32 / boxes;
         int pages = page_of(w, w.first * boxes + lane), next_pages = page_of(w, (w.first + ahead) * boxes + lane);
         int tiles_left = ahead;
+        // The next unit is asked for late: one taken over at the start would wait for
+        // the end of a long one while other CTAs run out of work.
+        if (steps < 2 && lane == 0) ask_next(smem_u32(&sh.next), smem_u32(&sh.next_full));
         for (int t = 0; t < 2 * steps; ++t) {
+          if (t == 2 * steps - 4 && lane == 0) ask_next(smem_u32(&sh.next), smem_u32(&sh.next_full));
           if (loaded >= S) {
             wait_or_abort(&sh.kv_empty[stage], phase ^ 1, abort);
             if (__any_sync(0xffffffffu, *abort)) break;
