@@ -102,17 +102,17 @@ PROTOTYPES = {
          _vp, _i64, _vp, ctypes.c_size_t, ctypes.c_uint, _int, _vp],
     ),
     "adb_prefill_workspace_size": (
-        _int, [_i64, _i64, _i64, _i64, _i64, _int, ctypes.POINTER(_size), ctypes.POINTER(_size)],
+        _int, [_i64, _i64, _i64, _i64, _i64, _i64, _int, ctypes.POINTER(_size)],
     ),
     "adb_prefill": (
         _int,
         [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
-         _vp, _size, _uint, _int, _vp],
+         _vp, _size, _int, _vp],
     ),
     "adb_prefill_paged": (
         _int,
         [_vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
-         _int, _vp, _size, _uint, _int, _vp],
+         _int, _vp, _size, _int, _vp],
     ),
     "adb_cache_write": (
         _int,

@@ -121,12 +121,19 @@ size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 // and the pairs of a sequence have half its tiles or more on average, so that
 // there are at most three times as many parts as SMs.
 struct Workspace {
-  int64_t slots, rows;
+  int64_t slots, rows;  // no slots: nothing can be cut into parts
   size_t off_ml, off_joins, off_count, bytes;
 };
 
-Workspace plan_workspace(int64_t total, int64_t group, int64_t dim, int64_t sms) {
-  Workspace w;
+// `max_keys`: of a sequence in the cache, or 0 for packed prompts.
+Workspace plan_workspace(int64_t total, int64_t kv_heads, int64_t group, int64_t dim, int64_t max_keys, int64_t sms) {
+  // Parts need a sequence of one and a half of the smallest.  The pairs of a
+  // prompt of n tokens have n / 256 tiles on average, so that its even share
+  // allows them only below a length.
+  const int64_t longest =
+      max_keys > 0 ? max_keys : std::min<int64_t>(total, 2 * (adb::kTile / group) * sms * 4 / (3 * kv_heads));
+  Workspace w = {};
+  if (longest <= (3 * adb::kMinPart / 2 - 1) * adb::kTile) return w;
   w.slots = 3 * sms;
   w.rows = std::min<int64_t>(2 * (adb::kTile / group), total) * group;
   w.off_ml = align256(static_cast<size_t>(w.slots * w.rows * dim) * sizeof(float));
@@ -166,8 +173,9 @@ int launch(adb::PrefillParams& p, const void* q, int64_t q_token, int64_t q_head
   // every sequence with a token may end in a partly filled pair of tiles
   const int64_t per = 2 * p.tile_tokens;
   const int64_t pairs = p.total / per + std::min(p.batch, p.total);
-  const Workspace ws = plan_workspace(p.total, p.group, dim, sms);
-  if (workspace == nullptr || !is_aligned(workspace, 256))
+  const int64_t max_keys = p.paged ? int64_t(p.max_blocks) << p.page_shift : 0;
+  const Workspace ws = plan_workspace(p.total, p.kv_heads, p.group, dim, max_keys, sms);
+  if (ws.slots > 0 && (workspace == nullptr || !is_aligned(workspace, 256)))
     return fail(ADB_ERR_WORKSPACE, "workspace must be a non-null 256-byte aligned device buffer");
   if (workspace_bytes < ws.bytes)
     return fail(ADB_ERR_WORKSPACE, "workspace too small: %zu bytes given, %zu needed", workspace_bytes, ws.bytes);
@@ -178,16 +186,10 @@ int launch(adb::PrefillParams& p, const void* q, int64_t q_token, int64_t q_head
   p.part_ml = reinterpret_cast<float2*>(base + ws.off_ml);
   p.joins = reinterpret_cast<adb::PrefillJoin*>(base + ws.off_joins);
   p.join_count = reinterpret_cast<int*>(base + ws.off_count);
-  // Splits need a sequence of one and a half parts.  The pairs of a prompt of n
-  // tokens have n / 256 tiles on average, so that its even share allows them
-  // only below a length.
-  const int64_t longest = p.paged ? int64_t(p.max_blocks) << p.page_shift
-                                  : std::min<int64_t>(p.total, 2 * p.tile_tokens * int64_t(sms) * 4 / (3 * p.kv_heads));
-  const bool splits = longest > (3 * adb::kMinPart / 2 - 1) * adb::kTile;
-  p.max_slots = splits ? static_cast<int>(ws.slots) : 0;
+  p.max_slots = static_cast<int>(ws.slots);
   // KV heads worked on at a time: even groups that keep the longest possible
   // sequence's K and V in L2
-  const int64_t keys = p.paged ? int64_t(p.max_blocks) << p.page_shift : p.total;
+  const int64_t keys = p.paged ? max_keys : p.total;
 const int64_t groups = std::min<int64_t>(p.kv_heads, (p.kv_heads * keys * dim * 4 + kL2Bytes - 1) / kL2Bytes);
   p.head_group = static_cast<int>((p.kv_heads + groups - 1) / groups);
   const int64_t grid = pairs * p.kv_heads + p.max_slots;
@@ -206,7 +208,7 @@ const int64_t groups = std::min<int64_t>(p.kv_heads, (p.kv_heads * keys * dim * 
   cudaError_t e = cudaLaunchKernelEx(&cfg, kernel.run, q_map, k_map, v_map, p);
   if (e != cudaSuccess) return cuda_fail(e, "prefill kernel launch");
   adb_host::count_launch();
-  if (!splits) return ADB_OK;
+  if (ws.slots == 0) return ADB_OK;
   const int64_t join_rows = ws.slots / 2 * ws.rows;
   cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(4 * sms, (join_rows + 7) / 8)));
   cfg.blockDim = dim3(adb::kJoinThreads);
@@ -222,24 +224,23 @@ const int64_t groups = std::min<int64_t>(p.kv_heads, (p.kv_heads * keys * dim * 
 extern "C" {
 
 int adb_prefill_workspace_size(int64_t total, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
-                               int device, size_t* bytes, size_t* header_bytes) {
+                               int64_t max_keys, int device, size_t* bytes) {
   if (bytes == nullptr) return fail(ADB_ERR_INVALID_ARGUMENT, "bytes pointer is null");
   const int rc = check_heads(total, batch, q_heads, kv_heads, head_dim);
   if (rc != ADB_OK) return rc;
+  if (max_keys < 0) return fail(ADB_ERR_INVALID_ARGUMENT, "max_keys must not be negative");
   int sms = 0;
   const int status = adb_host::sm_count(device, &sms);
   if (status != ADB_OK) return status;
-  const Workspace w = plan_workspace(total, q_heads / kv_heads, head_dim, sms);
-  *bytes = w.bytes;
-  if (header_bytes != nullptr) *header_bytes = 0;
+  *bytes = plan_workspace(total, kv_heads, q_heads / kv_heads, head_dim, max_keys, sms).bytes;
   return ADB_OK;
 }
 
 int adb_prefill(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
                 int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
                 const int32_t* cu_seqlens, void* out, int64_t total, int64_t batch, int64_t q_heads,
-                int64_t kv_heads, int64_t head_dim, void* workspace, size_t workspace_bytes, unsigned flags,
-                int device, void* stream) {
+                int64_t kv_heads, int64_t head_dim, void* workspace, size_t workspace_bytes, int device,
+                void* stream) {
   const int rc = check_heads(total, batch, q_heads, kv_heads, head_dim);
   if (rc != ADB_OK) return rc;
   if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || cu_seqlens == nullptr)
@@ -266,8 +267,8 @@ int adb_prefill_paged(const void* q, int64_t q_token_stride, int64_t q_head_stri
                       const void* v_cache, const int32_t* block_table, int64_t block_table_stride,
                       const int32_t* cu_seqlens, const int32_t* seqlens, void* out, int64_t total, int64_t batch,
                       int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t num_blocks, int64_t page_size,
-                      int64_t max_blocks_per_seq, int layout, void* workspace, size_t workspace_bytes,
-                      unsigned flags, int device, void* stream) {
+                      int64_t max_blocks_per_seq, int layout, void* workspace, size_t workspace_bytes, int device,
+                      void* stream) {
   const int rc = check_heads(total, batch, q_heads, kv_heads, head_dim);
   if (rc != ADB_OK) return rc;
   if (q == nullptr || k_cache == nullptr || v_cache == nullptr || out == nullptr)
@@ -281,9 +282,9 @@ int adb_prefill_paged(const void* q, int64_t q_token_stride, int64_t q_head_stri
                 (long long)page_size);
   if (num_blocks <= 0 || max_blocks_per_seq <= 0)
     return fail(ADB_ERR_INVALID_ARGUMENT, "num_blocks and max_blocks_per_seq must be positive");
-  if (num_blocks > INT32_MAX / kv_heads || max_blocks_per_seq > INT32_MAX / page_size)
+  if (num_blocks > INT32_MAX / kv_heads || max_blocks_per_seq > (1 << 30) / page_size)
     return fail(ADB_ERR_INVALID_ARGUMENT,
-                "num_blocks * kv_heads and max_blocks_per_seq * page_size must be below 2^31");
+                "num_blocks * kv_heads must be below 2^31, max_blocks_per_seq * page_size at most 2^30");
   if (block_table_stride < max_blocks_per_seq)
     return fail(ADB_ERR_INVALID_ARGUMENT, "block table row stride %lld is below max_blocks_per_seq %lld",
                 (long long)block_table_stride, (long long)max_blocks_per_seq);

@@ -508,7 +508,6 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       const int pad_tail = clamp_to(p.cu[p.batch], 0, p.total), pad_head = clamp_to(p.cu[0], 0, p.total);
       PrefillPlan plan;
       make_plan(p, plan);
-      if (p.max_slots > 0 && blockIdx.x == 0 && lane == 0) *p.join_count = plan.joins * p.kv_heads;
       const bool pads = pad_tail < p.total || pad_head > 0;
       const int boxes = p.paged ? max(1, kTile >> p.page_shift) : 1;
       const int box_rows = kTile / boxes;
@@ -527,6 +526,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       int index = blockIdx.x;
       bool go = true;
       for (int asked = 0; go; ++asked) {
+        if (p.max_slots > 0 && index == 0 && lane == 0) *p.join_count = plan.joins * p.kv_heads;
         PrefillWork w;
         find_work(p, plan, index, w);
         w.pad_head = pad_head;

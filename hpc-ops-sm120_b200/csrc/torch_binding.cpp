@@ -238,13 +238,19 @@ void check_devices(std::initializer_list<std::pair<const char*, const at::Tensor
   }
 }
 
-Call prepare_prefill(const at::Tensor& q, int64_t batch, int64_t kv_heads) {
-  const int device = q.get_device();
-  cudaStream_t stream = at::cuda::getCurrentCUDAStream(device).stream();
-  size_t total = 0, header = 0;
-  check_status(adb_prefill_workspace_size(q.size(0), batch, q.size(1), kv_heads, q.size(2), device, &total, &header));
-  return {device, stream, workspace_for(q, device, stream, total, header)};
+// Scratch from the caching allocator (it is given back in the stream's order;
+// a captured call's belongs to the graph's pool).
+at::Tensor prefill_workspace(const at::Tensor& q, int64_t batch, int64_t kv_heads, int64_t max_keys) {
+  size_t bytes = 0;
+  check_status(adb_prefill_workspace_size(q.size(0), batch, q.size(1), kv_heads, q.size(2), max_keys, q.get_device(),
+                                          &bytes));
+  return bytes > 0 ? at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte)) : at::Tensor();
 }
+
+size_t bytes_of(const at::Tensor& workspace) {
+  return workspace.defined() ? static_cast<size_t>(workspace.numel()) : 0;
+}
+void* data_of(const at::Tensor& workspace) { return workspace.defined() ? workspace.data_ptr() : nullptr; }
 
 at::Tensor prefill(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu_seqlens) {
   check_packed(q, "Q");
@@ -260,12 +266,13 @@ at::Tensor prefill(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v
   const int64_t batch = cu_seqlens.size(0) - 1;
   if (q.size(0) == 0 || batch == 0) return at::zeros({q.size(0), q.size(1), q.size(2)}, q.options());
   at::Tensor out = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
-  Call call = prepare_prefill(q, batch, k.size(1));
+  const int device = q.get_device();
+  const at::Tensor ws = prefill_workspace(q, batch, k.size(1), 0);
   check_status(adb_prefill(q.data_ptr(), token_stride(q), head_stride(q), k.data_ptr(), token_stride(k),
                            head_stride(k), v.data_ptr(), token_stride(v), head_stride(v),
                            cu_seqlens.data_ptr<int32_t>(), out.data_ptr(), q.size(0), batch, q.size(1), k.size(1),
-                           q.size(2), call.ws.buffer.data_ptr(), static_cast<size_t>(call.ws.buffer.numel()),
-                           call.ws.flags, call.device, call.stream));
+                           q.size(2), data_of(ws), bytes_of(ws), device,
+                           at::cuda::getCurrentCUDAStream(device).stream()));
   return out;
 }
 
@@ -285,14 +292,14 @@ at::Tensor prefill_paged(const at::Tensor& q, const at::Tensor& k_cache, const a
   const c10::cuda::CUDAGuard guard(q.device());
   at::Tensor out = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
   if (q.size(0) == 0) return out;
-  Call call = prepare_prefill(q, batch, pages.heads);
+  const int device = q.get_device();
+  const at::Tensor ws = prefill_workspace(q, batch, pages.heads, block_table.size(1) * pages.page);
   check_status(adb_prefill_paged(
       q.data_ptr(), token_stride(q), head_stride(q), k_cache.data_ptr(), v_cache.data_ptr(),
       block_table.data_ptr<int32_t>(), row_stride(block_table),
       cu_seqlens.data_ptr<int32_t>(), seqlens.data_ptr<int32_t>(), out.data_ptr(), q.size(0), batch, q.size(1),
       pages.heads, pages.dim, pages.blocks, pages.page, block_table.size(1), pages.layout,
-      call.ws.buffer.data_ptr(), static_cast<size_t>(call.ws.buffer.numel()), call.ws.flags, call.device,
-      call.stream));
+      data_of(ws), bytes_of(ws), device, at::cuda::getCurrentCUDAStream(device).stream()));
   return out;
 }
 

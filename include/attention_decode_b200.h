@@ -307,11 +307,13 @@ ADB_API int adb_decode_exchange_merged(const void* q, const void* k, const void*
 #define ADB_ERROR_FLAG_CACHE_FULL 32    /* no free page left for a row */
 #define ADB_ERROR_FLAG_CACHE_REFUSED 64 /* a row's request was refused */
 
-/* Workspace of adb_prefill and adb_prefill_paged for `total` rows (see
- * "Workspace" above). */
+/* Bytes of workspace that adb_prefill (max_keys = 0) or adb_prefill_paged
+ * (max_keys = max_blocks_per_seq * page_size) needs; 0 if it needs none.  It
+ * need not be zeroed and holds nothing between calls; calls that may run
+ * concurrently must use different ones. */
 ADB_API int adb_prefill_workspace_size(int64_t total, int64_t batch, int64_t q_heads,
-                                       int64_t kv_heads, int64_t head_dim, int device,
-                                       size_t* bytes, size_t* header_bytes);
+                                       int64_t kv_heads, int64_t head_dim, int64_t max_keys,
+                                       int device, size_t* bytes);
 
 /* Causal attention of whole prompts.  q [total, q_heads, head_dim], k and v
  * [total, kv_heads, head_dim], out [total, q_heads, head_dim] contiguous, all
@@ -321,8 +323,8 @@ ADB_API int adb_prefill(const void* q, int64_t q_token_stride, int64_t q_head_st
                         int64_t k_token_stride, int64_t k_head_stride, const void* v,
                         int64_t v_token_stride, int64_t v_head_stride, const int32_t* cu_seqlens,
                         void* out, int64_t total, int64_t batch, int64_t q_heads, int64_t kv_heads,
-                        int64_t head_dim, void* workspace, size_t workspace_bytes, unsigned flags,
-                        int device, void* stream);
+                        int64_t head_dim, void* workspace, size_t workspace_bytes, int device,
+                        void* stream);
 
 /* Causal attention of new tokens over a paged cache that already holds them
  * (adb_cache_write): sequence b has seqlens[b] tokens in its pages, the last
@@ -337,8 +339,8 @@ ADB_API int adb_prefill_paged(const void* q, int64_t q_token_stride, int64_t q_h
                               const int32_t* seqlens, void* out, int64_t total, int64_t batch,
                               int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                               int64_t num_blocks, int64_t page_size, int64_t max_blocks_per_seq,
-                              int layout, void* workspace, size_t workspace_bytes, unsigned flags,
-                              int device, void* stream);
+                              int layout, void* workspace, size_t workspace_bytes, int device,
+                              void* stream);
 
 /* Writes new tokens' K and V into their pages: token i of row b goes to
  * position starts[b] + i.  A token whose position has no page of the pool is

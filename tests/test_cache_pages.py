@@ -136,7 +136,7 @@ def state(gen, rows, longest, page, spare, device, width=None, share=True):
 @gpu
 @pytest.mark.parametrize("rows,longest,page,spare", (
     (1, 1, 8, 1), (1, 100, 8, 40), (7, 300, 16, 60), (33, 2000, 8, 3000), (300, 500, 64, 10), (3, 70000, 8, 20000),
-    (2500, 40, 8, 4000), (64, 5000, 256, 100),
+    (2500, 40, 8, 4000), (64, 5000, 256, 100), (20, 900, 8, 300000), (16384, 9, 8, 9000),
 ))
 @pytest.mark.parametrize("seed", (0, 1))
 def test_resize(rows, longest, page, spare, seed, device):
@@ -193,7 +193,7 @@ def test_resize_follows_no_bad_page(device):
 @gpu
 @pytest.mark.parametrize("rows,children,longest,page,spare", (
     (1, 1, 5, 8, 1), (2, 9, 100, 8, 4), (5, 40, 900, 16, 100), (8, 1500, 300, 64, 1400), (3, 30, 60000, 8, 29),
-    (40, 1, 33, 32, 0),
+    (40, 1, 33, 32, 0), (3, 16381, 20, 8, 16000), (4, 20, 5000, 8, 300000),
 ))
 def test_fork(rows, children, longest, page, spare, device):
     flags()
@@ -234,6 +234,7 @@ def test_fork_refuses(device):
 @gpu
 @pytest.mark.parametrize("rows,longest,page,spare", (
     (1, 1, 8, 0), (1, 1, 8, 1), (1, 0, 8, 7), (6, 200, 8, 33), (30, 1000, 16, 2000), (500, 100, 8, 1), (4, 90000, 8, 9000),
+    (30, 40000, 8, 250000),
 ))
 def test_compact(rows, longest, page, spare, device):
     flags()

@@ -56,7 +56,8 @@ def test_packed(lens, hq, hkv, dim, device):
 @gpu
 @pytest.mark.parametrize("hq,hkv,dim,lens", (
     (8, 2, 128, [5000]), (4, 4, 64, [2500, 3, 1111]), (2, 2, 128, [9001]), (32, 8, 128, [700] * 9 + [1]),
-    (8, 8, 128, [17] * 200), (7, 1, 64, [3, 2] * 700),
+    (8, 8, 128, [17] * 200), (7, 1, 64, [3, 2] * 700), (8, 2, 64, [0, 70] * 128), (8, 2, 64, [40] * 256 + [300]),
+    (8, 1, 128, [4000, 1, 1700]), (4, 1, 64, [2100]),
 ))
 def test_packed_long_or_many(hq, hkv, dim, lens, device):
     gen = torch.Generator(device).manual_seed(len(lens))
@@ -188,6 +189,10 @@ def test_paged(layout, page, hq, hkv, dim, device):
     ([600, 1, 1, 1], [9000, 17, 8000, 1], 8, 2, 128, 16),
     ([1] * 40, [50 * i + 1 for i in range(40)], 32, 8, 128, 32),
     ([200], [200], 4, 4, 128, 8),
+    ([500], [90], 4, 4, 64, 16),  # most rows see no key, the first tiles none at all
+    ([1] * 300 + [60], [7] * 300 + [5000], 4, 2, 64, 16),
+    ([40, 300], [20000, 3000], 8, 1, 128, 16),
+    ([2, 2, 2, 2], [1535, 1536, 1537, 40000], 2, 1, 64, 8),
 ))
 def test_paged_long_or_mixed(layout, new, total, hq, hkv, dim, page, device):
     gen = torch.Generator(device).manual_seed(sum(total))
@@ -438,7 +443,7 @@ def test_c_entry_points_refuse_on_the_host():
     p = 256  # an address that no refused call follows
 
     def packed(q=p, stride=512, total=6, batch=1, hq=8, hkv=2, dim=64, cu=p):
-        return lib.adb_prefill(q, stride, 64, p, 128, 64, p, 128, 64, cu, p, total, batch, hq, hkv, dim, p, 0, 0, 0, None)
+        return lib.adb_prefill(q, stride, 64, p, 128, 64, p, 128, 64, cu, p, total, batch, hq, hkv, dim, p, 0, 0, None)
 
     assert packed(q=None) == invalid and packed(cu=None) == invalid
     assert packed(q=264) == invalid and packed(stride=513) == invalid
@@ -448,11 +453,12 @@ def test_c_entry_points_refuse_on_the_host():
 
     def paged(table=p, page=8, layout=0, stride=4, blocks=9, width=4):
         return lib.adb_prefill_paged(p, 512, 64, p, p, table, stride, p, p, p, 6, 1, 8, 2, 64, blocks, page, width,
-                                     layout, p, 0, 0, 0, None)
+                                     layout, p, 0, 0, None)
 
     assert paged(table=None) == invalid and paged(layout=3) == invalid and paged(stride=3) == invalid
     assert paged(page=7) == unsupported and paged(page=24) == unsupported
     assert paged(blocks=0) == invalid and paged(blocks=2**30) == invalid and paged(width=2**28, stride=2**28) == invalid
     size = ctypes.c_size_t(0)
-    assert lib.adb_prefill_workspace_size(6, 1, 9, 2, 64, 0, ctypes.byref(size), None) == invalid
-    assert lib.adb_prefill_workspace_size(6, 1, 8, 2, 64, 0, None, None) == invalid
+    assert lib.adb_prefill_workspace_size(6, 1, 9, 2, 64, 0, 0, ctypes.byref(size)) == invalid
+    assert lib.adb_prefill_workspace_size(6, 1, 8, 2, 64, 0, 0, None) == invalid
+    assert lib.adb_prefill_workspace_size(6, 1, 8, 2, 64, -1, 0, ctypes.byref(size)) == invalid
