@@ -920,7 +920,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       const float inv = total == 0.f ? 0.f : 1.f / total;
       __nv_bfloat16* out = p.out + (static_cast<int64_t>(w.row0 + w.token0 + i * p.tile_tokens) * p.q_heads +
                                     w.head * p.group) * D;
-      const int64_t gap = static_cast<int64_t>(p.q_heads - p.group) * D;  // between the rows of two tokens
+      const int gap = (p.q_heads - p.group) * D;  // between the rows of two tokens (a tile's offsets fit 32 bits)
       const int rows = valid * p.group;
       const uint32_t mine = staging + i * C::kHalfBytes + (warp & 3) * 4096;
       if (w.parts > 1) {
@@ -957,6 +957,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         if (tid == 0 && w.part == 0)
           p.joins[w.join] = {w.row0 + w.token0, (w.valid[0] + w.valid[1]) * p.group, w.head, w.slot, w.parts};
       } else if ((warp & 3) * 32 < rows) {
+        int offset[8];  // of this lane's 16 bytes in eight stores, 4 rows each
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int r = (warp & 3) * 32 + 4 * k + (lane >> 3);
+          offset[k] = r < rows ? (r * p.group_magic >> 16) * gap + r * D + (lane & 7) * 8 : -1;
+        }
 #pragma unroll 1
         for (int c = 0; c < D; c += 64) {
 #pragma unroll
@@ -977,16 +983,15 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           __syncwarp();
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const int l = 4 * k + (lane >> 3), x = lane & 7, r = (warp & 3) * 32 + l;
+            const int l = 4 * k + (lane >> 3), x = lane & 7;
             const uint4 v = ld_shared_v4(mine + l * 128 + (x ^ (l & 7)) * 16);
-            if (r < rows)
-              *reinterpret_cast<uint4*>(out + (r * p.group_magic >> 16) * gap + static_cast<int64_t>(r) * D + c + x * 8) = v;
+            if (offset[k] >= 0) *reinterpret_cast<uint4*>(out + offset[k] + c) = v;
           }
           __syncwarp();
         }
         if (live && *reinterpret_cast<volatile int*>(&sh.fix[n & 1]) == n + 1)
           add_non_finite(p, w.seq, w.head, w.row0, D, w.open_keys, w.first * kTile + sees,
-                         out + token * gap + static_cast<int64_t>(row) * D, nullptr);
+                         out + token * gap + row * D, nullptr);
       }
       tcgen05_before_sync();
       work_done(n);
