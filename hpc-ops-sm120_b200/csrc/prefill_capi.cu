@@ -117,9 +117,8 @@ int prepare(int device) {
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 // Workspace, of nothing but parts: O, (maximum, total), the list of what to
-// join.  A part is two thirds of an SM's even share of all K/V tiles or more,
-// and the pairs of a sequence have half its tiles or more on average, so that
-// there are at most three times as many parts as SMs.
+// join.  The kernel makes at most as many more units by cutting as there are
+// SMs, so that at most twice as many are parts (a cut pair has two or more).
 struct Workspace {
   int64_t slots, rows;  // no slots: nothing can be cut into parts
   size_t off_ml, off_joins, off_count, bytes;
@@ -127,14 +126,14 @@ struct Workspace {
 
 // `max_keys`: of a sequence in the cache, or 0 for packed prompts.
 Workspace plan_workspace(int64_t total, int64_t kv_heads, int64_t group, int64_t dim, int64_t max_keys, int64_t sms) {
-  // Parts need a sequence of one and a half of the smallest.  The pairs of a
-  // prompt of n tokens have n / 256 tiles on average, so that its even share
-  // allows them only below a length.
+  // A cut needs a sequence of one and a half of the smallest parts.  The pairs
+  // of a prompt of n tokens have n / 256 tiles on average, so that only short
+  // prompts of few KV heads are longer than their even share.
   const int64_t longest =
       max_keys > 0 ? max_keys : std::min<int64_t>(total, 2 * (adb::kTile / group) * sms * 4 / (3 * kv_heads));
   Workspace w = {};
-  if (longest <= (3 * adb::kMinPart / 2 - 1) * adb::kTile) return w;
-  w.slots = 3 * sms;
+  if (longest <= (max_keys > 0 ? 3 * adb::kMinPart / 2 - 1 : 2 * adb::kMinPart) * adb::kTile) return w;
+  w.slots = 2 * sms;
   w.rows = std::min<int64_t>(2 * (adb::kTile / group), total) * group;
   w.off_ml = align256(static_cast<size_t>(w.slots * w.rows * dim) * sizeof(float));
   w.off_joins = w.off_ml + align256(static_cast<size_t>(w.slots * w.rows) * sizeof(float2));
@@ -192,7 +191,7 @@ int launch(adb::PrefillParams& p, const void* q, int64_t q_token, int64_t q_head
   const int64_t keys = p.paged ? max_keys : p.total;
 const int64_t groups = std::min<int64_t>(p.kv_heads, (p.kv_heads * keys * dim * 4 + kL2Bytes - 1) / kL2Bytes);
   p.head_group = static_cast<int>((p.kv_heads + groups - 1) / groups);
-  const int64_t grid = pairs * p.kv_heads + p.max_slots;
+  const int64_t grid = pairs * p.kv_heads + (ws.slots > 0 ? sms : 0);
   if (grid > INT32_MAX) return fail(ADB_ERR_INVALID_ARGUMENT, "too many tiles for one call");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));

@@ -209,23 +209,24 @@ __device__ __forceinline__ void make_plan(const PrefillParams& p, PrefillPlan& p
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, d);
     // ... or more, until the parts of more than half a share get an SM each (if
-    // there are no more pairs than SMs) and the workspace holds the parts
+    // there are no more pairs than SMs) and there are no more of them than the
+    // workspace and the grid have room for
     const bool few = __reduce_add_sync(0xffffffffu, units) * p.kv_heads <= p.sms;
     int share = max(kMinPart, static_cast<int>(fminf(ceilf(tiles * p.kv_heads / p.sms), 1e8f)));
     for (; p.max_slots > 0; share += share / 8 + 1) {
-      int slots = 0, large = 0;
+      int more = 0, large = 0;  // units that the cuts add, those of half a share or more
       units = 0;
 #pragma unroll
       for (int r = 0; r < kPlanRows; ++r) {
         if (32 * r >= p.batch) break;
         const int parts = max(1, (2 * plan.parts[r] + share) / (2 * share));
         units += plan.pairs[r] * parts;
-        if (parts > 1) slots += plan.pairs[r] * parts;
+        more += plan.pairs[r] * (parts - 1);
         if (2 * plan.parts[r] > share) large += plan.pairs[r] * parts;
       }
-      slots = __reduce_add_sync(0xffffffffu, slots);
+      more = __reduce_add_sync(0xffffffffu, more);
       large = __reduce_add_sync(0xffffffffu, large);
-      if (slots == 0 || (slots <= p.max_slots / p.kv_heads && !(few && large * p.kv_heads > p.sms))) break;
+      if (more == 0 || (more <= p.sms / p.kv_heads && !(few && large * p.kv_heads > p.sms))) break;
     }
 #pragma unroll
     for (int r = 0; r < kPlanRows; ++r) {
