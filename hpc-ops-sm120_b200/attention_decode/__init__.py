@@ -467,11 +467,18 @@ def combine_partials(acc, ml, out=None):
     return out
 
 
-def _tensors(**named):
-    Tensor = _torch().Tensor
-    for name, t in named.items():
-        if not isinstance(t, Tensor):
-            raise TypeError(f"{name} must be a tensor")
+def _call(function, *args, **tensors):
+    """The extension's ``function`` on the tensors and then ``args``, on the
+    current stream.  What is no tensor is looked for only when the binding has
+    refused the call: this runs on every step of a serving loop."""
+    try:
+        return function(*tensors.values(), *args)
+    except TypeError:
+        Tensor = _torch().Tensor
+        for name, t in tensors.items():
+            if not isinstance(t, Tensor):
+                raise TypeError(f"{name} must be a tensor") from None
+        raise
 
 
 def _nhd(layout) -> bool:
@@ -492,8 +499,7 @@ def attention_prefill(q, k, v, cu_seqlens):
     multiples of 8 elements.  Returns a new contiguous [T,Hq,D] BF16 tensor.
     Uses the current CUDA stream.
     """
-    _tensors(Q=q, K=k, V=v, cu_seqlens=cu_seqlens)
-    return _get_extension().prefill(q, k, v, cu_seqlens)
+    return _call(_get_extension().prefill, Q=q, K=k, V=v, cu_seqlens=cu_seqlens)
 
 
 def attention_prefill_paged(q, k_cache, v_cache, block_table, cu_seqlens, seqlens, *, layout="HND"):
@@ -509,8 +515,10 @@ def attention_prefill_paged(q, k_cache, v_cache, block_table, cu_seqlens, seqlen
     ``block_table`` and ``layout`` as for :func:`attention_decode_paged`, with
     Hq/Hkv from 1 to 64.  Returns a new contiguous [T,Hq,D] BF16 tensor.
     """
-    _tensors(Q=q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, cu_seqlens=cu_seqlens, seqlens=seqlens)
-    return _get_extension().prefill_paged(q, k_cache, v_cache, block_table, cu_seqlens, seqlens, _nhd(layout))
+    return _call(
+        _get_extension().prefill_paged, _nhd(layout), Q=q, k_cache=k_cache, v_cache=v_cache, block_table=block_table,
+        cu_seqlens=cu_seqlens, seqlens=seqlens,
+    )
 
 
 def cache_write(k, v, k_cache, v_cache, block_table, cu_seqlens, starts, *, layout="HND"):
@@ -522,8 +530,10 @@ def cache_write(k, v, k_cache, v_cache, block_table, cu_seqlens, starts, *, layo
     :func:`read_error_flag`.  Other slots, and so pages that rows share in
     full, are not touched.
     """
-    _tensors(K=k, V=v, k_cache=k_cache, v_cache=v_cache, block_table=block_table, cu_seqlens=cu_seqlens, starts=starts)
-    _get_extension().cache_write(k, v, k_cache, v_cache, block_table, cu_seqlens, starts, _nhd(layout))
+    _call(
+        _get_extension().cache_write, _nhd(layout), K=k, V=v, k_cache=k_cache, v_cache=v_cache, block_table=block_table,
+        cu_seqlens=cu_seqlens, starts=starts,
+    )
 
 
 def cache_copy_pages(k_cache, v_cache, src, dst):
@@ -536,8 +546,7 @@ def cache_copy_pages(k_cache, v_cache, src, dst):
     so a page may be the source of several, but the destination of one only,
     and no destination may be a source.
     """
-    _tensors(k_cache=k_cache, v_cache=v_cache, src=src, dst=dst)
-    _get_extension().cache_copy_pages(k_cache, v_cache, src, dst)
+    _call(_get_extension().cache_copy_pages, k_cache=k_cache, v_cache=v_cache, src=src, dst=dst)
 
 
 def cache_resize(block_table, seqlens, new_lens, page_refs, *, page_size):
@@ -555,8 +564,10 @@ def cache_resize(block_table, seqlens, new_lens, page_refs, *, page_size):
     used page which another row holds, since its next token would overwrite
     the other's (bit 64).  At most 16384 rows.
     """
-    _tensors(block_table=block_table, seqlens=seqlens, new_lens=new_lens, page_refs=page_refs)
-    return _get_extension().cache_resize(block_table, seqlens, new_lens, page_refs, page_size)
+    return _call(
+        _get_extension().cache_resize, page_size, block_table=block_table, seqlens=seqlens, new_lens=new_lens,
+        page_refs=page_refs,
+    )
 
 
 def cache_fork(block_table, seqlens, page_refs, parents, children, *, page_size):
@@ -572,8 +583,10 @@ def cache_fork(block_table, seqlens, page_refs, parents, children, *, page_size)
     was named before is refused (bit 64 of :func:`read_error_flag`); where no
     free page is left the child stays empty (bit 32).
     """
-    _tensors(block_table=block_table, seqlens=seqlens, page_refs=page_refs, parents=parents, children=children)
-    return _get_extension().cache_fork(block_table, seqlens, page_refs, parents, children, page_size)
+    return _call(
+        _get_extension().cache_fork, page_size, block_table=block_table, seqlens=seqlens, page_refs=page_refs,
+        parents=parents, children=children,
+    )
 
 
 def cache_compact(block_table, seqlens, page_refs, *, page_size):
@@ -585,8 +598,9 @@ def cache_compact(block_table, seqlens, page_refs, *, page_size):
     behind the last) are the copies that the caller makes for each layer
     (:func:`cache_copy_pages`) before it reads or writes the caches again.
     """
-    _tensors(block_table=block_table, seqlens=seqlens, page_refs=page_refs)
-    return _get_extension().cache_compact(block_table, seqlens, page_refs, page_size)
+    return _call(
+        _get_extension().cache_compact, page_size, block_table=block_table, seqlens=seqlens, page_refs=page_refs
+    )
 
 
 def read_error_flag(device=0, reset=True) -> int:

@@ -16,6 +16,7 @@
 #include <torch/extension.h>
 
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_runtime_api.h>
 
@@ -238,13 +239,20 @@ void check_devices(std::initializer_list<std::pair<const char*, const at::Tensor
   }
 }
 
+// An uninitialised tensor of t's type on its device; past the dispatcher, whose
+// share of a short call counts.
+at::Tensor empty_for(const at::Tensor& t, at::IntArrayRef sizes, at::ScalarType type) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, t.device(), c10::nullopt));
+}
+at::Tensor empty_for(const at::Tensor& t, at::IntArrayRef sizes) { return empty_for(t, sizes, t.scalar_type()); }
+
 // Scratch from the caching allocator (it is given back in the stream's order;
 // a captured call's belongs to the graph's pool).
 at::Tensor prefill_workspace(const at::Tensor& q, int64_t batch, int64_t kv_heads, int64_t max_keys) {
   size_t bytes = 0;
   check_status(adb_prefill_workspace_size(q.size(0), batch, q.size(1), kv_heads, q.size(2), max_keys, q.get_device(),
                                           &bytes));
-  return bytes > 0 ? at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte)) : at::Tensor();
+  return bytes > 0 ? empty_for(q, {static_cast<int64_t>(bytes)}, at::kByte) : at::Tensor();
 }
 
 size_t bytes_of(const at::Tensor& workspace) {
@@ -265,7 +273,7 @@ at::Tensor prefill(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v
   const c10::cuda::CUDAGuard guard(q.device());
   const int64_t batch = cu_seqlens.size(0) - 1;
   if (q.size(0) == 0 || batch == 0) return at::zeros({q.size(0), q.size(1), q.size(2)}, q.options());
-  at::Tensor out = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
+  at::Tensor out = empty_for(q, {q.size(0), q.size(1), q.size(2)});
   const int device = q.get_device();
   const at::Tensor ws = prefill_workspace(q, batch, k.size(1), 0);
   check_status(adb_prefill(q.data_ptr(), token_stride(q), head_stride(q), k.data_ptr(), token_stride(k),
@@ -290,7 +298,7 @@ at::Tensor prefill_paged(const at::Tensor& q, const at::Tensor& k_cache, const a
   check_devices({{"Q", &q}, {"k_cache", &k_cache}, {"v_cache", &v_cache}, {"block_table", &block_table},
                  {"cu_seqlens", &cu_seqlens}, {"seqlens", &seqlens}});
   const c10::cuda::CUDAGuard guard(q.device());
-  at::Tensor out = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
+  at::Tensor out = empty_for(q, {q.size(0), q.size(1), q.size(2)});
   if (q.size(0) == 0) return out;
   const int device = q.get_device();
   const at::Tensor ws = prefill_workspace(q, batch, pages.heads, block_table.size(1) * pages.page);
@@ -357,7 +365,7 @@ at::Tensor cache_resize(const at::Tensor& block_table, const at::Tensor& seqlens
                  {"page_refs", &page_refs}});
   const c10::cuda::CUDAGuard guard(block_table.device());
   const int device = block_table.get_device();
-  at::Tensor lens = at::empty_like(seqlens);
+  at::Tensor lens = empty_for(seqlens, {seqlens.size(0)});
   check_status(adb_cache_resize(block_table.data_ptr<int32_t>(), row_stride(block_table), seqlens.data_ptr<int32_t>(),
                                 new_lens.data_ptr<int32_t>(), page_refs.data_ptr<int32_t>(), lens.data_ptr<int32_t>(),
                                 block_table.size(0), page_refs.size(0), page_size, block_table.size(1), device,
@@ -375,9 +383,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> cache_fork(const at::Tensor& bloc
                  {"parents", &parents}, {"children", &children}});
   const c10::cuda::CUDAGuard guard(block_table.device());
   const int device = block_table.get_device();
-  at::Tensor src = at::empty_like(parents), dst = at::empty_like(parents);
+  at::Tensor src = empty_for(parents, {parents.size(0)}), dst = empty_for(parents, {parents.size(0)});
   if (parents.size(0) == 0) return {seqlens.clone(), src, dst};
-  at::Tensor lens = at::empty_like(seqlens);
+  at::Tensor lens = empty_for(seqlens, {seqlens.size(0)});
   check_status(adb_cache_fork(block_table.data_ptr<int32_t>(), row_stride(block_table), seqlens.data_ptr<int32_t>(),
                               page_refs.data_ptr<int32_t>(), parents.data_ptr<int32_t>(),
                               children.data_ptr<int32_t>(), parents.size(0), lens.data_ptr<int32_t>(),
@@ -394,8 +402,8 @@ std::tuple<at::Tensor, at::Tensor> cache_compact(const at::Tensor& block_table, 
   const c10::cuda::CUDAGuard guard(block_table.device());
   const int device = block_table.get_device();
   const int64_t blocks = page_refs.size(0);
-  at::Tensor src = at::empty({blocks / 2}, page_refs.options()), dst = at::empty({blocks / 2}, page_refs.options());
-  at::Tensor remap = at::empty({blocks}, page_refs.options());
+  at::Tensor src = empty_for(page_refs, {blocks / 2}), dst = empty_for(page_refs, {blocks / 2});
+  at::Tensor remap = empty_for(page_refs, {blocks});
   check_status(adb_cache_compact(block_table.data_ptr<int32_t>(), row_stride(block_table),
                                  seqlens.data_ptr<int32_t>(), page_refs.data_ptr<int32_t>(),
                                  src.data_ptr<int32_t>(), dst.data_ptr<int32_t>(), remap.data_ptr<int32_t>(),
