@@ -28,7 +28,8 @@ using adb_host::DeviceGuard;
 using adb_host::fail;
 using adb_host::is_aligned;
 
-constexpr int64_t kMaxRows = 16384;  // rows or forks of one bookkeeping call: their prefix sums live in shared memory
+constexpr int64_t kMaxRows = 16384;  // rows or forks of one bookkeeping call: three ints each in shared memory
+constexpr int kMaxBookSmem = 3 * kMaxRows * sizeof(int);
 
 int check_pages(int64_t page_size, int64_t num_blocks, int64_t max_blocks, int* shift) {
   if (page_size < 8 || page_size > (1 << 20) || (page_size & (page_size - 1)) != 0)
@@ -69,7 +70,8 @@ int launch(void (*kernel)(Args...), int64_t grid, int threads, size_t smem, int 
   if (rc != ADB_OK) return rc;
   cudaError_t e = cudaSuccess;
   if (smem > 48 * 1024) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    // always the same value: calls of other threads may come between this and the launch
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxBookSmem);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(max dynamic smem)");
   }
   cudaLaunchConfig_t cfg = {};

@@ -205,6 +205,28 @@ def test_paged_long_or_mixed(layout, new, total, hq, hkv, dim, page, device):
 
 
 @gpu
+@pytest.mark.parametrize("bad", (float("nan"), float("inf")))
+@pytest.mark.parametrize("at", (5, 9000, 19950, 19999))
+def test_non_finite_values_of_a_long_cache(at, bad, device):
+    """One KV head and few rows: the cache is cut into parts, `at` lies in the first, a middle or the last one."""
+    gen = torch.Generator(device).manual_seed(at)
+    new, total, hq, dim, page = 100, 20000, 4, 128, 16
+    k_cache, v_cache, table, tokens = make_pages(gen, [total], 1, dim, page, "HND", device)
+    q = randn(gen, new, hq, dim)
+    args = (table, ints([0, new], device), ints([total], device))
+    clean = ad.attention_prefill_paged(q, k_cache, v_cache, *args)
+    check_paged(clean, q, tokens, [new], [total])
+    v_cache[table[0, at // page].long(), 0, at % page, 33] = bad
+    out = ad.attention_prefill_paged(q, k_cache, v_cache, *args)
+    first = max(0, at - (total - new))  # first new token that sees it
+    touched = torch.zeros_like(out, dtype=torch.bool)
+    touched[first:, :, 33] = True
+    assert torch.equal(out[~touched], clean[~touched])
+    got = out[first:, :, 33].float()
+    assert torch.isnan(got).all() if math.isnan(bad) else (got == bad).all()
+
+
+@gpu
 def test_paged_agrees_with_decode(device):
     gen = torch.Generator(device).manual_seed(2)
     total = [1, 17, 1000, 4097, 64]
