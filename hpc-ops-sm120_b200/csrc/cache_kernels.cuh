@@ -234,6 +234,10 @@ __device__ __forceinline__ void let_go(const ResizeParams& p, Range range) {
   });
 }
 
+// 8 us for 32 rows that grow by a token, 17 us for 256 rows of which 30 end and
+// 212 grow in a pool of 66548 pages (one CTA-wide chunk per row and warp, without
+// the look ahead by lanes: 41 us).
+//
 // Steps: rows that end let their pages go; cuts are judged (refused where the
 // page that stays partly used is held by another row, whose tokens the row's
 // next ones would overwrite) and then made; the free pages are counted and
@@ -362,6 +366,8 @@ struct ForkParams {
   int batch, forks, max_blocks, num_blocks, page_shift;
 };
 
+// 6 us for 12 forks, 7 us for 248.
+//
 // A child shares its parent's full pages (they no longer change) and gets a
 // page of its own for the partly filled last one.  Each CTA keeps, redundantly,
 // which fork a row is the child of (the first that names it), the tokens that
@@ -474,6 +480,8 @@ struct CompactParams {
   int batch, max_blocks, num_blocks, page_shift;
 };
 
+// 6 us for 224 pages, 8.7 us for 6681 of which 1600 move.
+//
 // With n live pages, the i-th live page at or above n moves to the i-th free
 // page below n: the fewest copies that leave the live pages at the front, and
 // no page is both a source and a destination.
@@ -570,6 +578,9 @@ struct CopyParams {
 constexpr int kCopyThreads = 256;
 constexpr int kCopyVecs = 1024;  // of K and of V: 16 KB each per unit of work
 
+// Bound by HBM: 1600 pages of 32 KB in each pool take 29.7 us, 105 MB read and
+// as much written (7.1 TB/s, part of it in L2).
+//
 // One unit is a part of one entry's page, of K and of V.  The lists that
 // cache_compact returns are mostly -1 behind the moves, so each warp looks at
 // 32 of its CTA's units at a time and the CTA copies the valid ones.
@@ -636,6 +647,10 @@ constexpr int kWriteThreads = 256;
 constexpr int kWriteVecs = 2;         // of K and of V per thread
 constexpr int kWriteRows = 2048;      // rows whose offsets a block keeps in shared memory
 
+// Bound by HBM for prompts (6204 tokens, 50.7 MB moved: 9.6 us; 134 MB: 23.7 us,
+// 5.7 TB/s; 1 / 4 vectors per thread: 24.8 / 24.1 us), by latency for a step (32
+// tokens: 2.6 us behind another).
+//
 // A block takes `tokens` tokens.  The source loads do not depend on the places,
 // so they are issued first; meanwhile a thread per token finds its row, in
 // offsets that the block has read at once, and its page.

@@ -31,6 +31,13 @@
 // 8 r .. 8 r + 7 of all pages are one operand (pages are its stride): the keys
 // of a tile are taken in the order r, page, row (tile_key), in S, P and V alike.
 //
+// What bounds it: for long prompts the chain S -> softmax -> P V of a tile (3100
+// cycles per K/V tile for both tiles, 2048 of them tensor work) and the power
+// cap: 8192 tokens, 32/8 heads, D 128 take 420 us (1300 TFLOP/s) in 20 calls, 477
+// us in 1000; D 64 345 us.  For a few rows over a long cache the chain of one tile
+// (1.7 us) against 1.5 us of HBM time: one token over 131072, group 8, takes 110
+// us (4.9 TB/s).  A unit costs about 3 us outside its tile loop.
+//
 // Pipeline of a CTA (384 threads):
 //   warps 0-3, 4-7   softmax of tile 0, 1: one thread per row
 //   warp 8           finds the units; TMA loads: Q, then K_0 V_0 K_1 V_1 ...
@@ -58,9 +65,14 @@ namespace adb {
 
 constexpr int kPrefillThreads = 384;
 constexpr int kTile = 128;  // rows of a Q tile, keys of a K/V tile
-constexpr int kFirstPart = 64;  // keys whose weights are handed to the tensor cores before the others are computed
+// Keys whose weights are handed to the tensor cores before the others are
+// computed (32 / 64 / 96: 450 / 438 / 436 us on 8192 tokens, 32/8 heads, D 128,
+// and 396 / 368 / 381 us with D 64).
+constexpr int kFirstPart = 64;
 constexpr float kRescaleLog2 = 8.f;
-constexpr int kMinPart = 8;     // K/V tiles of a part, at least
+// K/V tiles of a part, at least (4 / 8: 71 / 63 us for 64 tokens over 16384,
+// 61 / 62 us for 8 sequences of up to 16384 with 1 to 5 new tokens).
+constexpr int kMinPart = 8;
 // Registers: 12 warps x 168 at launch; the loading and issuing warps give theirs to the softmax.
 constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
 static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * 168, "more registers than the block is launched with");
@@ -102,7 +114,7 @@ struct PrefillCfg {
   static constexpr int kHalves = D / 64;                     // 128-byte column blocks of a row
   static constexpr int kHalfBytes = kTile * 128;             // one column block of a tile
   static constexpr int kTileBytes = kHalves * kHalfBytes;
-  static constexpr int kStages = D == 128 ? 4 : 8;           // K and V tiles in flight
+  static constexpr int kStages = D == 128 ? 4 : 8;           // K and V tiles in flight (5 or 9: no faster)
   static constexpr int kSmemBytes = (2 + kStages) * kTileBytes + 2 * kHalfBytes + 1024;
 };
 
