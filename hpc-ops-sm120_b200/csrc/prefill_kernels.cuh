@@ -158,10 +158,14 @@ struct PrefillShared {
 
 __device__ __forceinline__ int clamp_to(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }
 
-// First row and row count of sequence b, whatever cu holds.
-__device__ __forceinline__ void sequence_rows(const PrefillParams& p, int b, int& first, int& count) {
-  first = clamp_to(p.cu[b], 0, p.total);
-  count = clamp_to(p.cu[b + 1], first, p.total) - first;
+// First row, row count and keys of sequence b, whatever cu and lens hold.
+struct Sequence {
+  int first, count, keys;
+};
+__device__ __forceinline__ Sequence load_sequence(const PrefillParams& p, int b) {
+  const int from = p.cu[b], to = p.cu[b + 1], len = p.paged ? p.lens[b] : 0;
+  const int first = clamp_to(from, 0, p.total), count = clamp_to(to, first, p.total) - first;
+  return {first, count, p.paged ? clamp_to(len, 0, p.max_blocks << p.page_shift) : count};
 }
 
 // The units of all sequences, held by one warp: lane l has sequences l, l + 32,
@@ -178,13 +182,10 @@ struct PrefillPlan {
   int joins;                       // pairs cut into parts
   int top;                         // highest level
   int scan_base, scan_before;      // where the walk stands
+  Sequence own;                    // sequence `lane`
 };
 
 __device__ __forceinline__ bool plan_is_sorted(const PrefillParams& p) { return p.batch <= 32 * kPlanRows; }
-
-__device__ __forceinline__ int sequence_keys(const PrefillParams& p, int b, int count) {
-  return p.paged ? clamp_to(p.lens[b], 0, p.max_blocks << p.page_shift) : count;
-}
 
 __device__ __forceinline__ int pairs_of(const PrefillParams& p, int count) {
   return static_cast<int>(static_cast<unsigned>(count + 2 * p.tile_tokens - 1) / static_cast<unsigned>(2 * p.tile_tokens));
@@ -195,6 +196,7 @@ __device__ __forceinline__ void make_plan(const PrefillParams& p, PrefillPlan& p
   plan.scan_base = plan.scan_before = plan.joins = 0;
   int units = 0, top = 0;
   float tiles = 0.f;  // K/V tiles of all pairs
+  plan.own = {0, 0, 0};
 #pragma unroll
   for (int r = 0; r < kPlanRows; ++r) plan.pairs[r] = plan.base[r] = 0, plan.parts[r] = 1;
   if (plan_is_sorted(p)) {
@@ -203,58 +205,59 @@ __device__ __forceinline__ void make_plan(const PrefillParams& p, PrefillPlan& p
       if (32 * r >= p.batch) break;
       const int b = 32 * r + lane;
       if (b < p.batch) {
-        int first, count;
-        sequence_rows(p, b, first, count);
-        plan.pairs[r] = pairs_of(p, count);
-        if (p.paged)
-          plan.base[r] = static_cast<int>(static_cast<unsigned>(max(sequence_keys(p, b, count) - count, 0)) /
-                                          static_cast<unsigned>(2 * p.tile_tokens));
+        const Sequence s = load_sequence(p, b);
+        if (r == 0) plan.own = s;
+        const int before = max(s.keys - s.count, 0);
+        plan.pairs[r] = pairs_of(p, s.count);
+        if (before > 0)
+          plan.base[r] = static_cast<int>(static_cast<unsigned>(before) / static_cast<unsigned>(2 * p.tile_tokens));
         units += plan.pairs[r];
         top = max(top, plan.base[r] + plan.pairs[r]);
         // for now the tiles of the sequence's last pair, its longest
-        const int keys = p.paged ? sequence_keys(p, b, count) : count;
-        plan.parts[r] = (keys + kTile - 1) / kTile;
-        tiles += 0.5f * plan.pairs[r] * (plan.parts[r] + (max(keys - count, 0) + kTile) / kTile);
+        plan.parts[r] = (s.keys + kTile - 1) / kTile;
+        tiles += 0.5f * plan.pairs[r] * (plan.parts[r] + (before + kTile) / kTile);
       }
     }
-    // parts of an SM's even share
+    if (p.max_slots > 0) {
+      // parts of an SM's even share
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, d);
-    // ... or more, until the parts of more than half a share get an SM each (if
-    // there are no more pairs than SMs) and there are no more of them than the
-    // workspace and the grid have room for
-    const bool few = __reduce_add_sync(0xffffffffu, units) * p.kv_heads <= p.sms;
-    int share = max(kMinPart, static_cast<int>(fminf(ceilf(tiles * p.kv_heads / p.sms), 1e8f)));
-    for (; p.max_slots > 0; share += share / 8 + 1) {
-      int more = 0, large = 0;  // units that the cuts add, those of half a share or more
-      units = 0;
+      for (int d = 16; d > 0; d >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, d);
+      // ... or more, until the parts of more than half a share get an SM each (if
+      // there are no more pairs than SMs) and there are no more of them than the
+      // workspace and the grid have room for
+      const bool few = __reduce_add_sync(0xffffffffu, units) * p.kv_heads <= p.sms;
+      int share = max(kMinPart, static_cast<int>(fminf(ceilf(__fdividef(tiles * p.kv_heads, p.sms)), 1e8f)));
+      for (;; share += share / 8 + 1) {
+        int more = 0, large = 0;  // units that the cuts add, those of half a share or more
+        units = 0;
+#pragma unroll
+        for (int r = 0; r < kPlanRows; ++r) {
+          if (32 * r >= p.batch) break;
+          const int parts = max(1, (2 * plan.parts[r] + share) / (2 * share));
+          units += plan.pairs[r] * parts;
+          more += plan.pairs[r] * (parts - 1);
+          if (2 * plan.parts[r] > share) large += plan.pairs[r] * parts;
+        }
+        more = __reduce_add_sync(0xffffffffu, more);
+        large = __reduce_add_sync(0xffffffffu, large);
+        if (more == 0 || (more <= p.sms / p.kv_heads && !(few && large * p.kv_heads > p.sms))) break;
+      }
 #pragma unroll
       for (int r = 0; r < kPlanRows; ++r) {
         if (32 * r >= p.batch) break;
-        const int parts = max(1, (2 * plan.parts[r] + share) / (2 * share));
-        units += plan.pairs[r] * parts;
-        more += plan.pairs[r] * (parts - 1);
-        if (2 * plan.parts[r] > share) large += plan.pairs[r] * parts;
+        plan.parts[r] = max(1, (2 * plan.parts[r] + share) / (2 * share));
+        if (plan.parts[r] > 1) {
+          plan.joins += plan.pairs[r];
+          plan.base[r] /= plan.parts[r];  // the order goes by a part's length
+          // (the highest level stays an upper bound)
+        }
       }
-      more = __reduce_add_sync(0xffffffffu, more);
-      large = __reduce_add_sync(0xffffffffu, large);
-      if (more == 0 || (more <= p.sms / p.kv_heads && !(few && large * p.kv_heads > p.sms))) break;
-    }
+    } else {
 #pragma unroll
-    for (int r = 0; r < kPlanRows; ++r) {
-      plan.parts[r] = p.max_slots > 0 ? max(1, (2 * plan.parts[r] + share) / (2 * share)) : 1;
-      if (plan.parts[r] > 1) {
-        plan.joins += plan.pairs[r];
-        plan.base[r] /= plan.parts[r];  // the order goes by a part's length
-        // (the highest level stays an upper bound)
-      }
+      for (int r = 0; r < kPlanRows; ++r) plan.parts[r] = 1;
     }
   } else {
-    for (int b = lane; b < p.batch; b += 32) {
-      int first, count;
-      sequence_rows(p, b, first, count);
-      units += pairs_of(p, count);
-    }
+    for (int b = lane; b < p.batch; b += 32) units += pairs_of(p, load_sequence(p, b).count);
   }
   plan.units = __reduce_add_sync(0xffffffffu, units);
   plan.top = __reduce_max_sync(0xffffffffu, top);
@@ -278,6 +281,14 @@ __device__ __forceinline__ void find_pair(const PrefillParams& p, PrefillPlan& p
   int& seq = w.seq;
   w.parts = 1;
   w.part = 0;
+  if (p.batch == 1) {
+    w.parts = __shfl_sync(0xffffffffu, plan.parts[0], 0);
+    const int i = w.parts == 1 ? r : r / w.parts;
+    seq = 0;
+    w.part = r - i * w.parts;
+    pair = __shfl_sync(0xffffffffu, plan.pairs[0], 0) - 1 - i;
+    return;
+  }
   if (plan_is_sorted(p)) {
     // lowest level with at most r pairs above it
     int lo = 0, hi = plan.top, above = 0;
@@ -317,9 +328,7 @@ __device__ __forceinline__ void find_pair(const PrefillParams& p, PrefillPlan& p
   if (r < plan.scan_before) plan.scan_base = plan.scan_before = 0;
   for (;;) {
     const int b = plan.scan_base + lane;
-    int first = 0, count = 0;
-    if (b < p.batch) sequence_rows(p, b, first, count);
-    const int mine = pairs_of(p, count);
+    const int mine = b < p.batch ? pairs_of(p, load_sequence(p, b).count) : 0;
     const int inc = warp_prefix(mine);
     const unsigned hit = __ballot_sync(0xffffffffu, r < plan.scan_before + inc);
     if (hit) {
@@ -354,13 +363,14 @@ __device__ __forceinline__ void find_work(const PrefillParams& p, PrefillPlan& p
   w.part = w.slot = w.join = 0;
   if (index >= plan.units * p.kv_heads) return;
   // (a group has to fill the GPU several times over: its last units leave SMs idle)
-  const int group = plan.units * p.head_group >= 4 * p.sms ? p.head_group : p.kv_heads;
-  const int heads0 = index / (plan.units * group) * group;
-  const int heads = min(group, p.kv_heads - heads0);
-  const int at = index - heads0 * plan.units;
-  w.head = heads0 + at % heads;
+  int heads0 = 0;
+  if (p.head_group < p.kv_heads && plan.units * p.head_group >= 4 * p.sms)
+    heads0 = index / (plan.units * p.head_group) * p.head_group;
+  const int heads = plan.units * p.head_group >= 4 * p.sms ? min(p.head_group, p.kv_heads - heads0) : p.kv_heads;
+  const int at = index - heads0 * plan.units, r = static_cast<int>(static_cast<unsigned>(at) / static_cast<unsigned>(heads));
+  w.head = heads0 + at - r * heads;
   int pair;
-  find_pair(p, plan, at / heads, w, pair);
+  find_pair(p, plan, r, w, pair);
   if (w.seq < 0) return;
   if (w.parts > 1) {
     // places in the workspace: those of the sequences before, then pair by pair
@@ -377,16 +387,23 @@ __device__ __forceinline__ void find_work(const PrefillParams& p, PrefillPlan& p
     w.slot = (slots + pair * w.parts) * p.kv_heads + w.head * w.parts;
     w.join = (pairs + pair) * p.kv_heads + w.head;
   }
-  int count;
-  sequence_rows(p, w.seq, w.row0, count);
-  w.keys = sequence_keys(p, w.seq, count);
-  w.before = w.keys - count;
+  Sequence s;
+  if (p.batch <= 32) {
+    s.first = __shfl_sync(0xffffffffu, plan.own.first, w.seq);
+    s.count = __shfl_sync(0xffffffffu, plan.own.count, w.seq);
+    s.keys = __shfl_sync(0xffffffffu, plan.own.keys, w.seq);
+  } else {
+    s = load_sequence(p, w.seq);
+  }
+  w.row0 = s.first;
+  w.keys = s.keys;
+  w.before = s.keys - s.count;
   w.token0 = pair * 2 * p.tile_tokens;
   w.open_keys = max(keys_of(w, w.token0), 0);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int t = w.token0 + i * p.tile_tokens;
-    w.valid[i] = clamp_to(count - t, 0, p.tile_tokens);
+    w.valid[i] = clamp_to(s.count - t, 0, p.tile_tokens);
     const int last = keys_of(w, t + w.valid[i] - 1);
     w.steps[i] = w.valid[i] > 0 && last > 0 ? (last + kTile - 1) / kTile : 0;
   }
