@@ -209,7 +209,7 @@ const int64_t groups = std::min<int64_t>(p.kv_heads, (p.kv_heads * keys * dim * 
   adb_host::count_launch();
   if (ws.slots == 0) return ADB_OK;
   const int64_t join_rows = ws.slots / 2 * ws.rows;
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(4 * sms, (join_rows + 7) / 8)));
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(2 * sms, (join_rows + 7) / 8)));
   cfg.blockDim = dim3(adb::kJoinThreads);
   cfg.dynamicSmemBytes = 0;
   e = cudaLaunchKernelEx(&cfg, dim == 128 ? adb::prefill_join_kernel<128> : adb::prefill_join_kernel<64>, p);
