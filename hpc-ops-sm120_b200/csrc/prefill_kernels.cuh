@@ -33,10 +33,10 @@
 //
 // What bounds it: for long prompts the chain S -> softmax -> P V of a tile (3100
 // cycles per K/V tile for both tiles, 2048 of them tensor work) and the power
-// cap: 8192 tokens, 32/8 heads, D 128 take 420 us (1300 TFLOP/s) in 20 calls, 477
+// cap: 8192 tokens, 32/8 heads, D 128 take 415 us (1320 TFLOP/s) in 20 calls, 475
 // us in 1000; D 64 345 us.  For a few rows over a long cache the chain of one tile
-// (1.7 us) against 1.5 us of HBM time: one token over 131072, group 8, takes 110
-// us (4.9 TB/s).  A unit costs about 3 us outside its tile loop.
+// (1.6 us) against 1.5 us of HBM time: one token over 131072, group 8, takes 103
+// us (5.2 TB/s).  A unit costs about 3 us outside its tile loop.
 //
 // Pipeline of a CTA (384 threads):
 //   warps 0-3, 4-7   softmax of tile 0, 1: one thread per row
@@ -48,6 +48,15 @@
 // reads its row of S_i, writes the weights P_i (BF16) over it, and the product
 // O_i += P_i V_j takes P_i from tensor memory.  While one tile's softmax runs
 // the tensor cores work on the other tile.
+//
+// P_i takes the first half of S_i's columns.  Where a unit has one tile only
+// (and always with D 64 and pages of 16) the next S's other half is computed as
+// soon as the first weights are handed over, and its keys' maximum is found
+// while the rest follows.  A product of 64 columns has the shared memory's rate
+// (three quarters of the time of 128), so with two tiles, which keep the tensor
+// cores busier, S comes at once.  Split / at once: 103 / 109 us for one token
+// over 131072, 226 / 243 for 256 rows of 1000, 447 / 427 for 8192 tokens, 999 /
+// 935 for 16384 tokens of 16/2 heads.
 //
 // The running maximum is raised (and O rescaled) only when it grows by more
 // than 2^8: until then weights up to 2^8 are exact enough in FP32 sums and in
@@ -146,7 +155,7 @@ struct PrefillShared {
   uint64_t work_full[2], work_empty[2];
   uint64_t q_full, q_empty;
   uint64_t kv_full[PrefillCfg<D>::kStages], kv_empty[PrefillCfg<D>::kStages];
-  uint64_t s_full[2], p_part[2], p_full[2], o_full[2];
+  uint64_t s_high[2], s_full[2], p_part[2], p_full[2], o_full[2];
   uint64_t v_turn[PrefillCfg<D>::kStages];   // a border tile of V is on its way
   uint64_t v_clean[PrefillCfg<D>::kStages];  // and cleared
   uint64_t fix_done[2];
@@ -498,6 +507,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     for (int i = 0; i < 2; ++i) {
       init(sh.work_full[i], 1);
       init(sh.work_empty[i], 11);
+      init(sh.s_high[i], 1);
       init(sh.s_full[i], 1);
       init(sh.p_part[i], 4);
       init(sh.p_full[i], 4);
@@ -665,26 +675,31 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       const uint64_t k_ring = kPair ? smem_desc_base(16, page_bytes) : k_major;
       const uint64_t v_ring = kPair ? smem_desc_base(page_bytes / 2, page_bytes) : smem_desc_base(C::kHalfBytes, 1024);
       const uint32_t k_half = (kPair ? page_bytes / 2 : C::kHalfBytes) >> 4;
-      constexpr uint32_t qk_idesc = mma_idesc(kTile, kTile, false);
-      constexpr uint32_t qk16_idesc = mma_idesc(kTile, kTile / 2, false);
+      constexpr uint32_t qk_idesc = mma_idesc(kTile, kTile, false), half_idesc = mma_idesc(kTile, kTile / 2, false);
       constexpr uint32_t pv_idesc = mma_idesc(kTile, D, true);
-      const auto qk = [&](int i, int stage) {
+      // from a tile's first 64 columns of S to its others: the second 8 rows of all pages, half of the pages, 64 keys
+      const uint32_t high = (pair16 ? 1024 : kPair ? (kTile / 2) * 256 : (kTile / 2) * 128) >> 4;
+      const auto qk_columns = [&](int i, int stage, int half, uint32_t idesc) {
         const uint64_t a = smem_desc(k_major, tiles + i * C::kTileBytes);
-        const uint64_t b = smem_desc(k_ring, ring + stage * C::kTileBytes);
+        const uint64_t b = smem_desc(k_ring, ring + stage * C::kTileBytes) + (half ? high : 0);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          mma_ss(tmem + i * kTile + half * (kTile / 2), a + ((k >> 2) * (C::kHalfBytes >> 4) + (k & 3) * 2),
+                 b + ((k >> 2) * k_half + (k & 3) * 2), idesc, k > 0);
+      };
+      const auto qk_high = [&](int i, int stage) {
         if (elect_one()) {
-          if (pair16) {
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-#pragma unroll
-              for (int k = 0; k < D / 16; ++k)
-                mma_ss(tmem + i * kTile + r * (kTile / 2), a + ((k >> 2) * (C::kHalfBytes >> 4) + (k & 3) * 2),
-                       b + (r * (1024 >> 4) + (k >> 2) * k_half + (k & 3) * 2), qk16_idesc, k > 0);
-          } else {
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-              mma_ss(tmem + i * kTile, a + ((k >> 2) * (C::kHalfBytes >> 4) + (k & 3) * 2),
-                     b + ((k >> 2) * k_half + (k & 3) * 2), qk_idesc, k > 0);
-          }
+          qk_columns(i, stage, 1, half_idesc);
+          mma_commit(smem_u32(&sh.s_high[i]));
+        }
+        __syncwarp();
+      };
+      // the first columns where qk_high has done the others, else all
+      const auto qk_rest = [&](int i, int stage, bool split) {
+        if (elect_one()) {
+          if (pair16 && !split) qk_columns(i, stage, 1, half_idesc);
+          qk_columns(i, stage, 0, split || pair16 ? half_idesc : qk_idesc);
+          if (!split) mma_commit(smem_u32(&sh.s_high[i]));
           mma_commit(smem_u32(&sh.s_full[i]));
         }
         __syncwarp();
@@ -715,12 +730,14 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         const int steps0 = sh.work[n & 1].steps[0], steps1 = sh.work[n & 1].steps[1], steps = max(steps0, steps1);
         if (steps > 0) {
           const int first_open = sh.work[n & 1].open_keys / kTile - sh.work[n & 1].first;
+          const bool split = D == 64 || pair16 || steps0 == 0 || steps1 == 0;
           wait_or_abort(&sh.q_full, q_phase, abort);
           q_phase ^= 1;
           wait_or_abort(&sh.kv_full[stage], phase, abort);
           tcgen05_after_sync();
-          if (steps0 > 0) qk(0, stage);
-          if (steps1 > 0) qk(1, stage);
+#pragma unroll 1  // less code: with both calls inlined 4 x 2048 tokens took 170 us, 165 so
+          for (int i = 0; i < 2; ++i)
+            if ((i ? steps1 : steps0) > 0) qk_rest(i, stage, false);
           commit(&sh.kv_empty[stage]);
           if (steps == 1) commit(&sh.q_empty);
           advance();
@@ -744,13 +761,14 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
               int& p_phase = i ? p_phase1 : p_phase0;
               wait_or_abort(&sh.p_part[i], p_phase, abort);
               tcgen05_after_sync();
+              if (split && j + 1 < mine) qk_high(i, k_stage);
               pv(i, v_stage, 0, kFirstPart / 16, j > 0);
               wait_or_abort(&sh.p_full[i], p_phase, abort);
               tcgen05_after_sync();
               p_phase ^= 1;
               pv(i, v_stage, kFirstPart / 16, kTile / 16, true);
               if (j + 1 < mine)
-                qk(i, k_stage);
+                qk_rest(i, k_stage, split);
               else
                 commit(&sh.o_full[i]);
             }
@@ -859,31 +877,34 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       const int sees = live ? all_see + token : 0;
       float top = -INFINITY, total = 0.f;
       for (int j = 0; j < steps; ++j) {
-        wait_or_abort(&sh.s_full[i], s_phase, abort);
-        s_phase ^= 1;
-        tcgen05_after_sync();
         float s[kTile];
-#pragma unroll
-        for (int c = 0; c < kTile; c += 32) tmem_ld32(s_at + c, s + c);
-        tmem_wait_ld();
-        if ((j + 1) * kTile > all_see) {
-          const int limit = sees - j * kTile;
-          if (kPair && p.page_shift == 4) {
-#pragma unroll
-            for (int c = 0; c < kTile; ++c) s[c] = tile_key16(c) < limit ? s[c] : -INFINITY;
-          } else {
-#pragma unroll
-            for (int c = 0; c < kTile; ++c) s[c] = c < limit ? s[c] : -INFINITY;
-          }
-        }
         float m0 = -INFINITY, m1 = m0, m2 = m0, m3 = m0;
 #pragma unroll
-        for (int c = 0; c < kTile; c += 8) {
-          m0 = max3(m0, s[c], s[c + 1]);
-          m1 = max3(m1, s[c + 2], s[c + 3]);
-          m2 = max3(m2, s[c + 4], s[c + 5]);
-          m3 = max3(m3, s[c + 6], s[c + 7]);
+        for (int c0 = kTile / 2; c0 >= 0; c0 -= kTile / 2) {
+          wait_or_abort(c0 > 0 ? &sh.s_high[i] : &sh.s_full[i], s_phase, abort);
+          tcgen05_after_sync();
+          tmem_ld32(s_at + c0, s + c0);
+          tmem_ld32(s_at + c0 + 32, s + c0 + 32);
+          tmem_wait_ld();
+          if ((j + 1) * kTile > all_see) {
+            const int limit = sees - j * kTile;
+            if (kPair && p.page_shift == 4) {
+#pragma unroll
+              for (int c = c0; c < c0 + kTile / 2; ++c) s[c] = tile_key16(c) < limit ? s[c] : -INFINITY;
+            } else {
+#pragma unroll
+              for (int c = c0; c < c0 + kTile / 2; ++c) s[c] = c < limit ? s[c] : -INFINITY;
+            }
+          }
+#pragma unroll
+          for (int c = c0; c < c0 + kTile / 2; c += 8) {
+            m0 = max3(m0, s[c], s[c + 1]);
+            m1 = max3(m1, s[c + 2], s[c + 3]);
+            m2 = max3(m2, s[c + 4], s[c + 5]);
+            m3 = max3(m3, s[c + 6], s[c + 7]);
+          }
         }
+        s_phase ^= 1;
         const float high = fmaxf(max3(m0, m1, m2), m3);
         if (j == 0) {
           top = high;
