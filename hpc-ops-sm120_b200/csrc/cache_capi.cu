@@ -110,6 +110,8 @@ int adb_cache_write(const void* k, int64_t k_token_stride, int64_t k_head_stride
     return fail(ADB_ERR_INVALID_ARGUMENT, "tokens, batch and KV heads must be positive");
   if (batch >= INT32_MAX || total > INT32_MAX)
     return fail(ADB_ERR_INVALID_ARGUMENT, "tokens and batch must be below 2^31");
+  if (kv_heads > (1 << 16))
+    return fail(ADB_ERR_UNSUPPORTED, "at most 65536 KV heads are supported (got %lld)", (long long)kv_heads);
   if (head_dim != 64 && head_dim != 128)
     return fail(ADB_ERR_UNSUPPORTED, "head dimension must be 64 or 128 (got %lld)", (long long)head_dim);
   int shift = 0;

@@ -383,3 +383,17 @@ def test_c_entry_points_refuse_on_the_host():
         return lib.adb_cache_copy_pages(k, p, p, p, count, 9, size, 0, None)
 
     assert copy(k=None) == invalid and copy(count=0) == invalid and copy(size=100) == invalid and copy(k=8) == invalid
+
+
+def test_write_refuses_more_heads_than_its_offsets_hold():
+    from attention_decode import _lib
+
+    lib = _lib.load_library()
+    p = 256  # an address that no refused call follows
+
+    def write(heads, blocks):
+        return lib.adb_cache_write(p, heads * 64, 64, p, heads * 64, 64, p, p, p, 4, p, p, 3, 2, heads, 64, blocks, 8, 4, 0, 0, None)
+
+    assert write(2**16 + 1, 9) == _lib.ADB_ERR_UNSUPPORTED and b"heads" in lib.adb_last_error()
+    assert write(2**40, 2**30) == _lib.ADB_ERR_UNSUPPORTED
+    assert write(2**16, 2**15) == _lib.ADB_ERR_INVALID_ARGUMENT  # num_blocks * heads
