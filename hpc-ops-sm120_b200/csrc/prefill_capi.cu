@@ -189,7 +189,7 @@ int launch(adb::PrefillParams& p, const void* q, int64_t q_token, int64_t q_head
   // KV heads worked on at a time: even groups that keep the longest possible
   // sequence's K and V in L2
   const int64_t keys = p.paged ? max_keys : p.total;
-const int64_t groups = std::min<int64_t>(p.kv_heads, (p.kv_heads * keys * dim * 4 + kL2Bytes - 1) / kL2Bytes);
+  const int64_t groups = std::min<int64_t>(p.kv_heads, (p.kv_heads * keys * dim * 4 + kL2Bytes - 1) / kL2Bytes);
   p.head_group = static_cast<int>((p.kv_heads + groups - 1) / groups);
   const int64_t grid = pairs * p.kv_heads + (ws.slots > 0 ? sms : 0);
   if (grid > INT32_MAX) return fail(ADB_ERR_INVALID_ARGUMENT, "too many tiles for one call");

@@ -1050,7 +1050,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   }
   __syncthreads();
   griddep_launch_dependents();
-  if (*abort != 0) __nanosleep(1000000);  // after a wait that ran out: what was still in flight
+  if (*abort != 0) {
+    // after a wait that ran out: parts are missing, so none are joined (the count
+    // was written at the start, long ago); and what was still in flight
+    if (tid == 0 && p.max_slots > 0) *p.join_count = 0;
+    __nanosleep(1000000);
+  }
   if (warp == 9) {
     tcgen05_after_sync();
     tmem_dealloc(tmem, 512);
