@@ -112,12 +112,23 @@ template <typename Pred>
 __device__ __forceinline__ PageBits find_pages(int num_blocks, Pred pred) {
   const int lane = threadIdx.x & 31;
   PageBits b{page_region(num_blocks), 0u, 0};
-#pragma unroll 8
-  for (int p = b.r.lo; p < b.r.hi; p += 32) {
-    const bool hit = p + lane < b.r.hi && pred(p + lane);
-    const unsigned hits = __ballot_sync(0xffffffffu, hit);
-    if (lane == (p - b.r.lo) >> 5) b.bits = hits;
-    b.count += __popc(hits);
+  if (b.r.hi - b.r.lo <= 32) {  // (the loop's code alone takes 1000 cycles to arrive)
+    b.bits = __ballot_sync(0xffffffffu, b.r.lo + lane < b.r.hi && pred(b.r.lo + lane));
+    b.count = __popc(b.bits);
+    return b;  // page_bits asks lane 0
+  }
+  constexpr int kAtOnce = 16;  // loads in flight
+  for (int p0 = b.r.lo; p0 < b.r.hi; p0 += 32 * kAtOnce) {
+    bool hit[kAtOnce];
+#pragma unroll
+    for (int x = 0; x < kAtOnce; ++x) hit[x] = p0 + 32 * x + lane < b.r.hi && pred(p0 + 32 * x + lane);
+#pragma unroll
+    for (int x = 0; x < kAtOnce; ++x) {
+      if (p0 + 32 * x >= b.r.hi) break;
+      const unsigned hits = __ballot_sync(0xffffffffu, hit[x]);
+      if (lane == ((p0 - b.r.lo) >> 5) + x) b.bits = hits;
+      b.count += __popc(hits);
+    }
   }
   return b;
 }
@@ -234,7 +245,7 @@ __device__ __forceinline__ void let_go(const ResizeParams& p, Range range) {
   });
 }
 
-// 8 us for 32 rows that grow by a token, 17 us for 256 rows of which 30 end and
+// 9 us for 32 rows that grow by a token, 16 us for 256 rows of which 30 end and
 // 212 grow in a pool of 66548 pages (one CTA-wide chunk per row and warp, without
 // the look ahead by lanes: 41 us).
 //
@@ -243,7 +254,7 @@ __device__ __forceinline__ void let_go(const ResizeParams& p, Range range) {
 // next ones would overwrite) and then made; the free pages are counted and
 // handed out, lowest first, to the growing rows in row order.  Steps that no
 // row asks for are skipped.
-__global__ void __cluster_dims__(kBookCtas, 1, 1) __launch_bounds__(kBookThreads)
+__global__ void __cluster_dims__(kBookCtas, 1, 1) __launch_bounds__(kBookThreads, 1)
     cache_resize_kernel(const ResizeParams p) {
   extern __shared__ int resize_smem[];
   int* prefix = resize_smem;             // [batch]: pages needed by the rows before
@@ -315,26 +326,40 @@ __global__ void __cluster_dims__(kBookCtas, 1, 1) __launch_bounds__(kBookThreads
     const PageBits free = find_pages(p.num_blocks, is_free);
     int rank = cluster_prefix<0>(free.count, sh);
     // Consecutive ranks are mostly of one row: the warp keeps the row of its last
-    // one, and each lane searches only where a row ends among the 32 pages.
+    // one, where its entries go and its last rank, and lanes search only where a
+    // row ends among the 32 pages.  (Eight SMs issue this loop for the whole pool:
+    // with the row's values read again for every 32 pages it took 10400 cycles for
+    // 256 rows and 66548 pages, so 7300.)
     int row = rank < needed ? last_at_most(prefix, 0, p.batch - 1, rank) : 0;
+    int row_end = -1;  // none kept yet
+    bool granted = false;
+    int32_t* entries = nullptr;  // of rank 0, if the row had it
     for (int at = free.r.lo; at < free.r.hi && rank < needed; at += 32) {
       const unsigned hits = page_bits(free, at, is_free);
-      if (hits == 0) continue;
       const int mine = rank + __popc(hits & ((1u << lane) - 1));
-      const int row1 = row + 1 == p.batch || prefix[row + 1] > rank + __popc(hits) - 1
-                           ? row
-                           : last_at_most(prefix, row, p.batch - 1, rank + __popc(hits) - 1);
+      rank += __popc(hits);
+      if (rank <= row_end) {
+        if ((hits >> lane & 1) && granted) {
+          entries[mine] = at + lane;
+          p.refs[at + lane] = 1;
+        }
+        continue;
+      }
+      if (hits == 0) continue;
       const int row0 = row;
-      row = row1;
+      row = last_at_most(prefix, row0, p.batch - 1, rank - 1);
       if ((hits >> lane & 1) && mine < needed) {
-        const int b = last_at_most(prefix, row0, row1, mine);
+        const int b = last_at_most(prefix, row0, row, mine);
         const int first = pages(olds[b]), last = pages(wants[b]);
         if (prefix[b] + (last - first) <= sh.all) {
           p.table[b * p.stride + first + mine - prefix[b]] = at + lane;
           p.refs[at + lane] = 1;
         }
       }
-      rank += __popc(hits);
+      const int first = pages(olds[row]);
+      row_end = prefix[row] + pages(wants[row]) - first;
+      granted = row_end <= sh.all;
+      entries = p.table + row * p.stride + (first - prefix[row]);
     }
   }
   for (int b = all_tid; b < p.batch; b += kBookCtas * kBookThreads) {
@@ -372,7 +397,7 @@ struct ForkParams {
 // page of its own for the partly filled last one.  Each CTA keeps, redundantly,
 // which fork a row is the child of (the first that names it), the tokens that
 // each fork takes over and the prefix sum of the pages needed.
-__global__ void __cluster_dims__(kBookCtas, 1, 1) __launch_bounds__(kBookThreads)
+__global__ void __cluster_dims__(kBookCtas, 1, 1) __launch_bounds__(kBookThreads, 1)
     cache_fork_kernel(const ForkParams p) {
   extern __shared__ int fork_smem[];
   int* prefix = fork_smem;               // [forks]
@@ -485,7 +510,7 @@ struct CompactParams {
 // With n live pages, the i-th live page at or above n moves to the i-th free
 // page below n: the fewest copies that leave the live pages at the front, and
 // no page is both a source and a destination.
-__global__ void __cluster_dims__(kBookCtas, 1, 1) __launch_bounds__(kBookThreads)
+__global__ void __cluster_dims__(kBookCtas, 1, 1) __launch_bounds__(kBookThreads, 1)
     cache_compact_kernel(const CompactParams p) {
   __shared__ BookShared sh;
   const int tid = threadIdx.x, lane = tid & 31;
