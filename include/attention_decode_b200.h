@@ -345,7 +345,8 @@ ADB_API int adb_prefill_paged(const void* q, int64_t q_token_stride, int64_t q_h
 /* Writes new tokens' K and V into their pages: token i of row b goes to
  * position starts[b] + i.  A token whose position has no page of the pool is
  * not written and sets ADB_ERROR_FLAG_CACHE_PAGE.  The slots written must be
- * distinct (no two rows hold the same page at a position that is written). */
+ * distinct (no two rows hold the same page at a position that is written).
+ * At most 65536 KV heads. */
 ADB_API int adb_cache_write(const void* k, int64_t k_token_stride, int64_t k_head_stride,
                             const void* v, int64_t v_token_stride, int64_t v_head_stride,
                             void* k_cache, void* v_cache, const int32_t* block_table,
