@@ -1000,9 +1000,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           }
           if (live) {
             p.part_ml[first_row + row] = make_float2(top, total);
+            // Only those of the part's own keys: the join multiplies by 0 what a row has
+            // of a part that it sees nothing of, and 0 * infinity is NaN.
             if (*reinterpret_cast<volatile int*>(&sh.fix[n & 1]) == n + 1)
-              add_non_finite(p, w.seq, w.head, w.row0, D, w.open_keys, w.first * kTile + sees, out,
-                             p.part_o + (first_row + row) * D);
+              add_non_finite(p, w.seq, w.head, w.row0, D, max(w.open_keys, w.first * kTile),
+                             w.first * kTile + min(sees, steps * kTile), out, p.part_o + (first_row + row) * D);
           }
         }
         if (tid == 0 && w.part == 0)

@@ -227,6 +227,36 @@ def test_non_finite_values_of_a_long_cache(at, bad, device):
 
 
 @gpu
+@pytest.mark.parametrize("bad", (float("nan"), float("inf"), -float("inf")))
+@pytest.mark.parametrize("hq,hkv,dim,page,new,total,seen,later,border", (
+    (8, 8, 128, 16, 256, 8260, 8010, 8100, 8064), (8, 8, 64, 64, 256, 9316, 9100, 9300, 9216),
+    (8, 2, 128, 8, 64, 9246, 9200, 9230, 9216), (8, 2, 64, 32, 64, 9246, 9200, 9230, 9216),
+))
+def test_non_finite_values_on_both_sides_of_a_part(hq, hkv, dim, page, new, total, seen, later, border, bad, device):
+    """The last part starts at key `border`, among the new tokens: rows between see `seen`, no key of that part, and not
+    its non-finite value either."""
+    gen = torch.Generator(device).manual_seed(total)
+    k_cache, v_cache, table, tokens = make_pages(gen, [total], hkv, dim, page, "HND", device)
+    q = randn(gen, new, hq, dim)
+    args = (table, ints([0, new], device), ints([total], device))
+    clean = ad.attention_prefill_paged(q, k_cache, v_cache, *args)
+    check_paged(clean, q, tokens, [new], [total])
+    head, heads = hkv - 1, slice((hkv - 1) * (hq // hkv), hq)
+    for key, column in ((seen, 33), (later, 50)):
+        v_cache[table[0, key // page].long(), head, key % page, column] = bad
+    out = ad.attention_prefill_paged(q, k_cache, v_cache, *args)
+    touched = torch.zeros_like(out, dtype=torch.bool)
+    first = {}
+    for key, column in ((seen, 33), (later, 50)):
+        first[column] = key - (total - new)
+        touched[first[column] :, heads, column] = True
+    assert first[33] < border - (total - new) <= first[50]
+    assert torch.equal(out[~touched], clean[~touched])
+    got = out[touched].float()
+    assert torch.isnan(got).all() if math.isnan(bad) else (got == bad).all()
+
+
+@gpu
 def test_paged_agrees_with_decode(device):
     gen = torch.Generator(device).manual_seed(2)
     total = [1, 17, 1000, 4097, 64]
