@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "attention_decode_b200.h"
 #include "cache_kernels.cuh"
@@ -58,6 +59,22 @@ int check_rows(const void* table, int64_t stride, const void* lens, int64_t batc
   return ADB_OK;
 }
 
+// Once per device: the shared memory that the rows of a resize or fork may take.
+// Whatever this call's size: beyond 48 KB in all a kernel needs the permission,
+// and beside its dynamic part it has a static one.
+int prepare(int device) {
+  static std::atomic<uint64_t> done{0};
+  const uint64_t bit = uint64_t(1) << device;
+  if (done.load(std::memory_order_acquire) & bit) return ADB_OK;
+  for (const void* kernel : {reinterpret_cast<const void*>(&adb::cache_resize_kernel),
+                             reinterpret_cast<const void*>(&adb::cache_fork_kernel)}) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxBookSmem);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(max dynamic smem)");
+  }
+  done.fetch_or(bit, std::memory_order_release);
+  return ADB_OK;
+}
+
 // Launches `kernel` with programmatic stream serialisation (it waits for the
 // kernels before it itself).
 template <typename... Args>
@@ -66,14 +83,9 @@ int launch(void (*kernel)(Args...), int64_t grid, int threads, size_t smem, int 
   DeviceGuard guard(device);
   if (guard.error != cudaSuccess) return cuda_fail(guard.error, "cudaSetDevice");
   int sms = 0;
-  const int rc = adb_host::sm_count(device, &sms);
+  int rc = adb_host::sm_count(device, &sms);
+  if (rc == ADB_OK && smem > 0) rc = prepare(device);
   if (rc != ADB_OK) return rc;
-  cudaError_t e = cudaSuccess;
-  if (smem > 48 * 1024) {
-    // always the same value: calls of other threads may come between this and the launch
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxBookSmem);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(max dynamic smem)");
-  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(static_cast<unsigned>(threads));
@@ -84,7 +96,7 @@ int launch(void (*kernel)(Args...), int64_t grid, int threads, size_t smem, int 
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
   if (e != cudaSuccess) return cuda_fail(e, what);
   adb_host::count_launch();
   return ADB_OK;

@@ -4,6 +4,10 @@ results have to be equal."""
 
 from __future__ import annotations
 
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -208,6 +212,17 @@ def test_fork(rows, children, longest, page, spare, device):
     assert got.tolist() == after and got_src.tolist() == src and got_dst.tolist() == dst
     assert dev_table.tolist() == table and dev_refs.tolist() == refs
     assert flags() == bits
+
+
+@gpu
+@pytest.mark.parametrize("call,sizes", (
+    ("resize", ("4084", "4085", "4095", "4096", "4097")), ("fork", ("4084,4084", "4085,4084", "4095,4096", "4096,4096", "4097,4096")),
+))
+def test_rows_around_48_kb_of_shared_memory(call, sizes, device):
+    """Three ints per row, or one per row and two per fork, beside what the kernel has of its own."""
+    child = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cache_rows_child.py")
+    proc = subprocess.run([sys.executable, child, call, *sizes], capture_output=True, text=True, timeout=600)
+    assert proc.returncode == 0 and proc.stdout.split() == ["ok"], proc.stderr[-4000:]
 
 
 @gpu
