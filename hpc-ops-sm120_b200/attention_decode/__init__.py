@@ -581,7 +581,9 @@ def cache_fork(block_table, seqlens, page_refs, parents, children, *, page_size)
     layer.  ``lens`` are the lengths after.  Parents' lengths are those before
     the call.  A row index outside the table, a child that is not empty or
     was named before is refused (bit 64 of :func:`read_error_flag`); where no
-    free page is left the child stays empty (bit 32).
+    free page is left the child stays empty (bit 32).  A parent's entry outside
+    the pool sets bit 16: a full page's is passed on as it is, and a last
+    page's content is not copied.  At most 16384 rows and 16384 forks.
     """
     return _call(
         _get_extension().cache_fork, page_size, block_table=block_table, seqlens=seqlens, page_refs=page_refs,
@@ -596,7 +598,8 @@ def cache_compact(block_table, seqlens, page_refs, *, page_size):
     ``block_table`` and ``page_refs`` name the new places when the call is
     done; ``src, dst = cache_compact(...)`` (int32 [num_blocks // 2], -1
     behind the last) are the copies that the caller makes for each layer
-    (:func:`cache_copy_pages`) before it reads or writes the caches again.
+    (:func:`cache_copy_pages`) before it reads or writes the caches again.  At
+    most 16384 rows.
     """
     return _call(
         _get_extension().cache_compact, page_size, block_table=block_table, seqlens=seqlens, page_refs=page_refs

@@ -450,8 +450,11 @@ __global__ void __cluster_dims__(kBookCtas, 1, 1) __launch_bounds__(kBookThreads
       // forks without a copy repeat the next prefix: the last one at `mine` is the one that needs it
       const int i = last_at_most(prefix, 0, p.forks - 1, mine);
       const int full = tokens[i] >> p.page_shift;
-      p.src[i] = p.table[p.parents[i] * p.stride + full];
-      p.dst[i] = at + lane;
+      const int page = p.table[p.parents[i] * p.stride + full];
+      const bool in = static_cast<unsigned>(page) < static_cast<unsigned>(p.num_blocks);
+      if (!in) atomicOr(&g_adb_error_flag, kErrCachePage);
+      p.src[i] = in ? page : -1;
+      p.dst[i] = in ? at + lane : -1;
       p.table[p.children[i] * p.stride + full] = at + lane;
       p.refs[at + lane] = 1;
     }

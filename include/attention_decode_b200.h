@@ -390,7 +390,9 @@ ADB_API int adb_cache_resize(int32_t* block_table, int64_t block_table_stride,
  * src[i] -> dst[i] (adb_cache_copy_pages, once per layer; -1, -1 where there
  * is nothing to copy).  Lengths are those before the call.  Refused: a row
  * index outside the table, a child that is not empty, a child named before.
- * Forks that find no free page, in order, leave their child empty. */
+ * Forks that find no free page, in order, leave their child empty.  A parent's
+ * entry outside the pool sets ADB_ERROR_FLAG_CACHE_PAGE: a full page's is
+ * passed on as it is, and a last page's content is not copied. */
 ADB_API int adb_cache_fork(int32_t* block_table, int64_t block_table_stride, const int32_t* seqlens,
                            int32_t* page_refs, const int32_t* parents, const int32_t* children,
                            int64_t forks, int32_t* lens_out, int32_t* src, int32_t* dst,

@@ -226,6 +226,18 @@ def test_rows_around_48_kb_of_shared_memory(call, sizes, device):
 
 
 @gpu
+@pytest.mark.parametrize("page", (-1, -5, 9, 2**31 - 1))
+def test_fork_follows_no_bad_page(page, device):
+    """The parent's last, partly filled page is none of the pool: the child's own has no source."""
+    flags()
+    table, refs = ints([[3, page, -1], [-1, -1, -1]], device), ints([0, 0, 0, 1, 0, 0, 0, 0, 0], device)
+    lens, src, dst = ad.cache_fork(table, ints([12, 0], device), refs, ints([0], device), ints([1], device), page_size=8)
+    assert flags() == 16
+    assert lens.tolist() == [12, 12] and src.tolist() == [-1] and dst.tolist() == [-1]
+    assert table.tolist() == [[3, page, -1], [3, 0, -1]] and refs.tolist() == [1, 0, 0, 2, 0, 0, 0, 0, 0]
+
+
+@gpu
 def test_fork_refuses(device):
     """A child named twice, one that is not empty, rows that are not there, a row as its own child; a parent that is
     a child of the same call counts as empty."""
