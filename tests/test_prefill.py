@@ -226,6 +226,65 @@ def test_non_finite_values_of_a_long_cache(at, bad, device):
     assert torch.isnan(got).all() if math.isnan(bad) else (got == bad).all()
 
 
+def scored(gen, heights, hq, hkv, dim):
+    """q, k, v of which key j has a score of about heights[j], for every row."""
+    n = len(heights)
+    u = torch.randint(2, (dim,), generator=gen, device=gen.device).float() * 2 - 1
+    q = (u * (1 + 0.25 * torch.randn(n, hq, dim, generator=gen, device=gen.device))).bfloat16()
+    k = u * (heights.to(gen.device) / math.sqrt(dim))[:, None, None]
+    k = (k + 0.5 * torch.randn(n, hkv, dim, generator=gen, device=gen.device)).bfloat16()
+    return q, k, randn(gen, n, hkv, dim)
+
+
+def heights(kind, n):
+    """Scores that make the running maximum grow by far more than a factor of 2^8, several times, or not at all."""
+    j = torch.arange(n).float()
+    if kind == "rising":
+        return -40 + 80 * torch.floor(12 * j / n) / 12
+    if kind == "falling":
+        return 40 - 80 * torch.floor(12 * j / n) / 12
+    if kind == "waves":
+        return 30 * torch.sin(j * (20 / n))
+    at = {"first": 5, "middle": n // 2 - 100, "last": n - 10}[kind]
+    return torch.where(j == at, 130.0, 0.0)  # by itself, whatever the others' weights: less than 2^-149 of its own
+
+
+KINDS = ("rising", "falling", "waves", "first", "middle", "last")
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hq,hkv,dim,lens", (
+    (8, 2, 128, [700, 400]), (4, 4, 64, [900, 400]), (32, 4, 64, [500]), (2, 2, 128, [3000]), (4, 1, 64, [3500]),
+))
+def test_packed_growing_scores(kind, hq, hkv, dim, lens, device):
+    gen = torch.Generator(device).manual_seed(lens[0])
+    q, k, v = scored(gen, torch.cat([heights(kind, n) for n in lens]), hq, hkv, dim)
+    check_packed(ad.attention_prefill(q, k, v, ints(offsets(lens), device)), q, k, v, lens)
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("page", (8, 16, 64))
+@pytest.mark.parametrize("hq,hkv,dim,new,total", (
+    (8, 2, 128, 150, 1100), (8, 8, 64, 150, 1100), (8, 2, 128, 3, 1100), (16, 2, 64, 3, 1100),
+    (4, 1, 128, 100, 20000), (8, 1, 64, 5, 20000), (2, 2, 128, 200, 9000),
+))
+def test_paged_growing_scores(kind, page, hq, hkv, dim, new, total, device):
+    """One and two tiles of rows, whole and cut into parts."""
+    gen = torch.Generator(device).manual_seed(total + new)
+    q, k, v = scored(gen, heights(kind, total), hq, hkv, dim)
+    blocks = ref.pages_of(total, page)
+    order = torch.randperm(blocks, generator=gen, device=device)
+    caches = [torch.full((blocks, page, hkv, dim), float("nan"), dtype=torch.bfloat16, device=device) for _ in range(2)]
+    at = torch.arange(total, device=device)
+    for cache, x in zip(caches, (k, v)):
+        cache[order[at // page], at % page] = x
+    args = (*caches, order.int()[None], ints([0, new], device), ints([total], device))
+    out = ad.attention_prefill_paged(q[-new:].contiguous(), *args, layout="NHD")
+    check_paged(out, q[-new:], [(k, v)], [new], [total])
+
+
 @gpu
 @pytest.mark.parametrize("bad", (float("nan"), float("inf"), -float("inf")))
 @pytest.mark.parametrize("hq,hkv,dim,page,new,total,seen,later,border", (
