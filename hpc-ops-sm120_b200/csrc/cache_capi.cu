@@ -83,7 +83,7 @@ int launch(void (*kernel)(Args...), int64_t grid, int threads, size_t smem, int 
   DeviceGuard guard(device);
   if (guard.error != cudaSuccess) return cuda_fail(guard.error, "cudaSetDevice");
   int sms = 0;
-  int rc = adb_host::sm_count(device, &sms);
+  int rc = adb_host::sm_count(device, &sms);  // refuses other devices
   if (rc == ADB_OK && smem > 0) rc = prepare(device);
   if (rc != ADB_OK) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -137,10 +137,13 @@ int adb_cache_write(const void* k, int64_t k_token_stride, int64_t k_head_stride
   if (!is_aligned(k, 16) || !is_aligned(v, 16) || !is_aligned(k_cache, 16) || !is_aligned(v_cache, 16) ||
       ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7) != 0)
     return fail(ADB_ERR_INVALID_ARGUMENT, "K, V and caches must be 16-byte aligned, strides multiples of 8 elements");
+  int sms = 0;
+  const int status = adb_host::sm_count(device, &sms);
+  if (status != ADB_OK) return status;
   // tokens per block: as many as fill its threads' loads, fewer where the GPU would not be filled
   const int64_t vecs = kv_heads * (head_dim / 8);
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(adb::kWriteThreads, adb::kWriteThreads * adb::kWriteVecs / vecs));
-  const int64_t tokens = std::max<int64_t>(1, std::min<int64_t>(most, total / (2 * 148)));
+  const int64_t tokens = std::max<int64_t>(1, std::min<int64_t>(most, total / (2 * sms)));
   const int64_t blocks = (total + tokens - 1) / tokens;
   adb::WriteParams p;
   p.k = static_cast<const __nv_bfloat16*>(k);
@@ -186,7 +189,10 @@ int adb_cache_copy_pages(void* k_cache, void* v_cache, const int32_t* src, const
   if (chunks > INT32_MAX) return fail(ADB_ERR_INVALID_ARGUMENT, "page too large");
   p.chunks = static_cast<int>(chunks);
   p.num_blocks = static_cast<int>(num_blocks);
-  const int64_t grid = std::min<int64_t>(count * chunks, 148 * 8);
+  int sms = 0;
+  const int rc = adb_host::sm_count(device, &sms);
+  if (rc != ADB_OK) return rc;
+  const int64_t grid = std::min<int64_t>(count * chunks, 8 * sms);
   return launch(&adb::cache_copy_pages_kernel, grid, adb::kCopyThreads, 0, device, stream, "page copy launch", p);
 }
 
