@@ -245,9 +245,10 @@ __device__ __forceinline__ void let_go(const ResizeParams& p, Range range) {
   });
 }
 
-// 9 us for 32 rows that grow by a token, 16 us for 256 rows of which 30 end and
+// 8 us for 32 rows that grow by a token, 15 us for 256 rows of which 30 end and
 // 212 grow in a pool of 66548 pages (one CTA-wide chunk per row and warp, without
-// the look ahead by lanes: 41 us).
+// the look ahead by lanes: 33 us).  Here and below: in a graph of 20 calls, without
+// the copies that bring the state back.
 //
 // Steps: rows that end let their pages go; cuts are judged (refused where the
 // page that stays partly used is held by another row, whose tokens the row's
@@ -508,7 +509,7 @@ struct CompactParams {
   int batch, max_blocks, num_blocks, page_shift;
 };
 
-// 6 us for 224 pages, 8.7 us for 6681 of which 1600 move.
+// 6 us for 224 pages, 7 us for 6681 of which 1600 move.
 //
 // With n live pages, the i-th live page at or above n moves to the i-th free
 // page below n: the fewest copies that leave the live pages at the front, and
@@ -606,8 +607,8 @@ struct CopyParams {
 constexpr int kCopyThreads = 256;
 constexpr int kCopyVecs = 1024;  // of K and of V: 16 KB each per unit of work
 
-// Bound by HBM: 1600 pages of 32 KB in each pool take 29.7 us, 105 MB read and
-// as much written (7.1 TB/s, part of it in L2).
+// Bound by HBM: 1607 pages of 32 KB in each pool take 35 us, 105 MB read and as
+// much written (6.0 TB/s).
 //
 // One unit is a part of one entry's page, of K and of V.  The lists that
 // cache_compact returns are mostly -1 behind the moves, so each warp looks at

@@ -18,9 +18,9 @@
 // control), so that one CTA's loads and first products overlap the end of its
 // unit before.  Units that see the most keys come first.
 //
-// Splits.  Where a sequence's K/V tiles are one and a half times an SM's even
-// share of all tiles or more (few rows over a long cache), its pairs are cut
-// into parts of about that share.  A part leaves its unnormalised O and
+// Splits.  In batches of up to 256 sequences, where a sequence's K/V tiles are
+// one and a half times an SM's even share of all tiles or more (few rows over a
+// long cache), its pairs are cut into parts of about that share.  A part leaves its unnormalised O and
 // (maximum, total) in the workspace, and a second kernel joins them, a warp per
 // row.  (Joined in the CTA of the part that finishes last, 256 rows of 16 parts
 // took 45 us.)
@@ -55,8 +55,13 @@
 // while the rest follows.  A product of 64 columns has the shared memory's rate
 // (three quarters of the time of 128), so with two tiles, which keep the tensor
 // cores busier, S comes at once.  Split / at once: 103 / 109 us for one token
-// over 131072, 226 / 243 for 256 rows of 1000, 447 / 427 for 8192 tokens, 999 /
-// 935 for 16384 tokens of 16/2 heads.
+// over 131072, 226 / 243 for 256 rows of 1000, 445 / 427 for 8192 tokens and
+// 849 / 808 for 16384 tokens of 16/2 heads (20 calls after a pause; 496 / 475
+// and 958 / 913 in 1000).
+//
+// The weights are rounded to BF16 for the product (half a step is 2^-8 of a
+// weight): A and B of a product have one type, and V is BF16.  The total sums
+// the unrounded weights; it, the maximum and O are FP32 throughout, parts too.
 //
 // The running maximum is raised (and O rescaled) only when it grows by more
 // than 2^8: until then weights up to 2^8 are exact enough in FP32 sums and in
@@ -181,8 +186,10 @@ __device__ __forceinline__ Sequence load_sequence(const PrefillParams& p, int b)
 // ...  Pair i of a sequence is on level base + i + 1, the keys that it sees in
 // units of a pair's tokens, and higher levels come first: with counts F(l) of
 // the pairs above a level, a pair is found by bisection and no list is needed.
-// Larger batches, whose many sequences fill the GPU in any order, are walked
-// in their order.
+// Larger batches are walked in their order and nothing is cut, so that one CTA
+// per KV head streams a long cache among them: 300 single tokens, one over 131072
+// and the others over 500, 64/8 heads, D 128, take 1503 us, 250 take 245.  (300
+// prompts, 299 of 100 tokens and then one of 8192: 588 us, 250 of them 578.)
 constexpr int kPlanRows = 8;
 struct PrefillPlan {
   int pairs[kPlanRows], base[kPlanRows];
